@@ -1,5 +1,6 @@
 // [pccl-amd extension] Kernel-level entry points used by the test-suite and micro-benchmarks (not part of pccl.h).
 // dtype arguments use the CCoIP wire encoding (pccl::DType), op uses pccl::ReduceOp, algo uses pccl::QuantAlgo.
+#include <algorithm>
 #include <chrono>
 #include <cstring>
 #include <mutex>
@@ -7,6 +8,7 @@
 
 #include "../common/device_backend.hpp"
 #include "../kernels/host_kernels.hpp"
+#include "../kernels/muon_common.hpp"
 #include "../kernels/optim_common.hpp"
 
 using namespace pccl;
@@ -256,4 +258,146 @@ PCCLX_EXPORT int pcclxOuterSgd(float *outer, float *mom, const float *pg, void *
     DeviceBackend *be = device_backend();
     if (!be) return -1;
     return be->outer_sgd(outer, mom, pg, local, count, lt, p, nullptr) && be->device_sync() ? 0 : -1;
+}
+
+// Log probabilities of given tokens (csrc/kernels/logprob_common.hpp), asynchronous on `stream` of the current device.
+// Returns 0, -1 (no device backend, or the launch failed) or -2 (arguments).
+PCCLX_EXPORT int pcclxTokenLogprobs(const void *logits, int64_t row_stride, int64_t rows, int64_t vocab, int dtype,
+                                    const int64_t *targets, int64_t ignore_index, int top_k, float *logprob,
+                                    float *entropy, float *stats, float *top_logprob, int64_t *top_index,
+                                    void *stream) {
+    DeviceBackend *be = device_backend();
+    if (!be) return -1;
+    if (rows < 0 || rows > INT32_MAX || vocab < 1 || vocab > INT32_MAX || top_k < 0 ||
+        top_k > kernels::kMaxTopLogprobs || top_k > vocab)
+        return -2;
+    const kernels::LogprobArgs a{logits,  row_stride, rows,  vocab,       targets,  ignore_index,
+                                 top_k,   logprob,    entropy, stats, top_logprob, top_index};
+    return be->token_logprobs(a, static_cast<DType>(dtype), stream) ? 0 : -1;
+}
+
+// Gradient of pcclxTokenLogprobs with respect to the logits; g_* may be null (no gradient from that result).
+PCCLX_EXPORT int pcclxTokenLogprobsGrad(const void *logits, int64_t row_stride, int64_t rows, int64_t vocab, int dtype,
+                                        const int64_t *targets, int64_t ignore_index, int top_k,
+                                        const float *entropy, const float *stats, const int64_t *top_index,
+                                        const float *g_logprob, const float *g_entropy, const float *g_top,
+                                        void *d_logits, void *stream) {
+    DeviceBackend *be = device_backend();
+    if (!be) return -1;
+    if (rows < 0 || rows > INT32_MAX || vocab < 1 || vocab > INT32_MAX || top_k < 0 ||
+        top_k > kernels::kMaxTopLogprobs || top_k > vocab)
+        return -2;
+    kernels::LogprobGradArgs g;
+    g.fwd = {logits, row_stride, rows, vocab, targets, ignore_index, top_k, nullptr, const_cast<float *>(entropy),
+             const_cast<float *>(stats), nullptr, const_cast<int64_t *>(top_index)};
+    g.g_logprob = g_logprob;
+    g.g_entropy = g_entropy;
+    g.g_top = g_top;
+    g.d_logits = d_logits;
+    return be->token_logprobs_grad(g, static_cast<DType>(dtype), stream) ? 0 : -1;
+}
+
+namespace {
+
+// entries of a call: shapes[3 i ..] = count, rows, cols; false if a size is out of range
+bool muon_entries(int n, const int64_t *shapes, std::vector<kernels::MuonEntry> &out) {
+    constexpr int64_t kMax = INT32_MAX - kernels::kMuonPad;
+    for (int i = 0; i < n; ++i) {
+        const int64_t count = shapes[3 * i], rows = shapes[3 * i + 1], cols = shapes[3 * i + 2];
+        if (count < 0 || rows < 0 || cols < 0 || count > kMax || rows > kMax || cols > kMax) return false;
+        kernels::MuonEntry e;
+        e.count = static_cast<int>(count);
+        e.rows = static_cast<int>(rows);
+        e.cols = static_cast<int>(cols);
+        out.push_back(e);
+    }
+    return true;
+}
+
+struct Span {
+    uintptr_t from, to;
+    bool written;
+};
+
+// a written tensor that shares memory with another one of the call
+bool spans_collide(std::vector<Span> &v) {
+    std::sort(v.begin(), v.end(), [](const Span &a, const Span &b) { return a.from < b.from; });
+    uintptr_t end = 0, written_end = 0; // furthest end so far, of any span / of the written ones
+    for (const Span &s : v) {
+        if (s.from < written_end || (s.written && s.from < end)) return true;
+        end = std::max(end, s.to);
+        if (s.written) written_end = std::max(written_end, s.to);
+    }
+    return false;
+}
+
+} // namespace
+
+// Bytes of workspace pcclxMuon needs for n entries of (count, rows, cols); -1: sizes out of range.
+PCCLX_EXPORT int64_t pcclxMuonWorkspace(int n, const int64_t *shapes) {
+    try {
+        std::vector<kernels::MuonEntry> entries;
+        if (n < 0 || !muon_entries(n, shapes, entries)) return -1;
+        return static_cast<int64_t>(kernels::muon_plan(entries, 1, 1, nullptr));
+    } catch (...) {
+        return -1;
+    }
+}
+
+// Orthogonalises (mom = null) or takes a Muon step on n entries of `count` contiguous row-major matrices each
+// (csrc/kernels/muon_common.hpp), asynchronously on `stream` of the current device. w[i] may be g[i] itself where
+// types agree; otherwise nothing written may overlap anything else. Returns 0, -1 (no backend / launch failed), -2
+// (arguments), -3 (overlap).
+PCCLX_EXPORT int pcclxMuon(int n, const int64_t *shapes, const void *const *g, int gtype, void *const *w, int wtype,
+                           float *const *mom, const float *alpha, double decay, double momentum, int nesterov,
+                           int steps, const float *coefficients, double eps, void *workspace, int64_t workspace_bytes,
+                           void *stream) {
+    try {
+        const auto gt = static_cast<DType>(gtype), wt = static_cast<DType>(wtype);
+        const auto ok_type = [](DType t) { return t == DType::F32 || t == DType::BF16 || t == DType::F16; };
+        if (n < 0 || steps < 1 || !ok_type(gt) || !ok_type(wt)) return -2;
+        std::vector<kernels::MuonEntry> entries;
+        if (!muon_entries(n, shapes, entries)) return -2;
+        std::vector<Span> spans;
+        for (int i = 0; i < n; ++i) {
+            auto &e = entries[i];
+            e.g = g[i];
+            e.w = w[i];
+            e.mom = mom ? mom[i] : nullptr;
+            e.alpha = alpha ? alpha[i] : 0.0f;
+            const size_t elems = static_cast<size_t>(e.count) * e.rows * e.cols;
+            if (elems == 0) continue;
+            const auto span = [&](const void *p, size_t es, bool written) {
+                const auto from = reinterpret_cast<uintptr_t>(p);
+                spans.push_back({from, from + elems * es, written});
+            };
+            const bool in_place = !mom && e.g == e.w && gt == wt;
+            if (!in_place) span(e.g, dtype_size(gt), false);
+            span(e.w, dtype_size(wt), true);
+            if (mom) span(e.mom, sizeof(float), true);
+        }
+        if (spans_collide(spans)) return -3;
+        std::vector<std::vector<kernels::MuonEntry>> groups;
+        const size_t need = kernels::muon_plan(entries, dtype_size(gt), dtype_size(wt), &groups);
+        if (workspace_bytes < 0 || static_cast<size_t>(workspace_bytes) < need ||
+            reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+            return -2;
+        if (groups.empty()) return 0;
+        DeviceBackend *be = device_backend();
+        if (!be) return -1;
+        kernels::MuonParams p;
+        p.steps = steps;
+        p.a = coefficients[0];
+        p.b = coefficients[1];
+        p.c = coefficients[2];
+        p.eps = eps;
+        p.momentum = static_cast<float>(momentum);
+        p.decay = static_cast<float>(decay);
+        p.nesterov = nesterov;
+        for (const auto &group : groups)
+            if (!be->muon(group.data(), static_cast<int>(group.size()), gt, wt, p, workspace, stream)) return -1;
+        return 0;
+    } catch (...) {
+        return -1;
+    }
 }

@@ -7,6 +7,8 @@
 #include <cstddef>
 #include <cstdint>
 
+#include "../kernels/logprob_common.hpp"
+#include "../kernels/muon_common.hpp"
 #include "../kernels/optim_common.hpp"
 #include "../kernels/quant_common.hpp"
 #include "types.hpp"
@@ -131,6 +133,16 @@ public:
                              DevStream s) = 0;
     virtual bool outer_sgd(float *outer, float *mom, const float *pg, void *local, size_t count, DType local_t,
                            const kernels::OuterSgdParams &p, DevStream s) = 0;
+
+    // log probabilities of given tokens and their gradient (csrc/kernels/logprob_common.hpp); logits F32/BF16/F16
+    virtual bool token_logprobs(const kernels::LogprobArgs &, DType, DevStream) { return false; }
+    virtual bool token_logprobs_grad(const kernels::LogprobGradArgs &, DType, DevStream) { return false; }
+
+    // one group of kernels::muon_plan: orthogonalise, or the whole Muon step (csrc/kernels/muon_common.hpp); gt / wt:
+    // F32/BF16/F16 types of the gradients / of the parameters or results
+    virtual bool muon(const kernels::MuonEntry *, int, DType, DType, const kernels::MuonParams &, void *, DevStream) {
+        return false;
+    }
 };
 
 // Waits for `e` by polling with short sleeps (2 us doubling to 100 us) instead of the runtime's synchronize, which

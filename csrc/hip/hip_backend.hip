@@ -386,6 +386,16 @@ public:
                    const kernels::OuterSgdParams &p, DevStream s) override {
         return hipk::launch_outer_sgd(outer, mom, pg, local, count, lt, p, static_cast<hipStream_t>(s));
     }
+    bool token_logprobs(const kernels::LogprobArgs &a, DType t, DevStream s) override {
+        return hipk::launch_token_logprobs(a, t, static_cast<hipStream_t>(s));
+    }
+    bool token_logprobs_grad(const kernels::LogprobGradArgs &a, DType t, DevStream s) override {
+        return hipk::launch_token_logprobs_grad(a, t, static_cast<hipStream_t>(s));
+    }
+    bool muon(const kernels::MuonEntry *entries, int n, DType gt, DType wt, const kernels::MuonParams &p, void *ws,
+              DevStream s) override {
+        return hipk::launch_muon(entries, n, gt, wt, p, ws, static_cast<hipStream_t>(s));
+    }
 
 private:
     struct VmmMap {

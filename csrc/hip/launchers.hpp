@@ -8,6 +8,8 @@
 #include <cstdint>
 
 #include "../common/types.hpp"
+#include "../kernels/logprob_common.hpp"
+#include "../kernels/muon_common.hpp"
 #include "../kernels/optim_common.hpp"
 #include "../kernels/quant_common.hpp"
 
@@ -39,6 +41,14 @@ bool launch_multi_gather(void *dst, const void *const *srcs, const size_t *offse
 bool launch_pseudo_grad(float *pg, const float *outer, const void *local, size_t count, DType lt, hipStream_t s);
 bool launch_outer_sgd(float *outer, float *mom, const float *pg, void *local, size_t count, DType lt,
                       const kernels::OuterSgdParams &p, hipStream_t s);
+
+// hip_logprob.hip
+bool launch_token_logprobs(const kernels::LogprobArgs &a, DType t, hipStream_t s);
+bool launch_token_logprobs_grad(const kernels::LogprobGradArgs &a, DType t, hipStream_t s);
+
+// hip_muon.hip: one group of muon_plan
+bool launch_muon(const kernels::MuonEntry *entries, int n, DType gt, DType wt, const kernels::MuonParams &p, void *ws,
+                 hipStream_t s);
 
 // hip_hash.hip
 bool launch_simplehash(const void *dev_ptr, size_t n_bytes, uint32_t *partial_scratch, uint32_t *out, hipStream_t s);

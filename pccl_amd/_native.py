@@ -7,8 +7,8 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import (POINTER, Structure, c_bool, c_char_p, c_double, c_float, c_int, c_size_t, c_uint8, c_uint16, c_uint32,
-                    c_uint64, c_void_p)
+from ctypes import (POINTER, Structure, c_bool, c_char_p, c_double, c_float, c_int, c_int64, c_size_t, c_uint8, c_uint16,
+                    c_uint32, c_uint64, c_void_p)
 
 try:  # share torch's HIP runtime with the plugin
     import torch  # noqa: F401
@@ -164,6 +164,15 @@ def _load() -> ctypes.CDLL:
         "pcclxPseudoGrad": ([c_void_p, c_void_p, c_void_p, c_size_t, c_int, c_int], c_int),
         "pcclxOuterSgd": ([c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_int, c_float, c_float, c_float, c_float,
                            c_int, c_int, c_int], c_int),
+        # token log probabilities (pccl_amd.ops.logprobs)
+        "pcclxTokenLogprobs": ([c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p,
+                                c_void_p, c_void_p, c_void_p, c_void_p, c_void_p], c_int),
+        "pcclxTokenLogprobsGrad": ([c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p,
+                                    c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p], c_int),
+        # Newton-Schulz orthogonalisation and the Muon step (pccl_amd.ops.muon)
+        "pcclxMuonWorkspace": ([c_int, p(c_int64)], c_int64),
+        "pcclxMuon": ([c_int, p(c_int64), p(c_void_p), c_int, p(c_void_p), c_int, p(c_void_p), p(c_float), c_double,
+                       c_double, c_int, c_int, p(c_float), c_double, c_void_p, c_int64, c_void_p], c_int),
         # shareable (VMM + fd) device memory and xGMI/IPC buffer-mode counters (pccl_amd.memory)
         "pcclxShareableQuery": ([c_void_p, c_size_t, p(c_uint64), p(c_size_t)], c_int),
         "pcclxShareableLiveBytes": ([], c_size_t),

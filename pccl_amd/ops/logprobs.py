@@ -1,0 +1,174 @@
+"""Log probabilities of given tokens, with the row's entropy and its top alternatives, differentiable.
+
+The loss of a language model (``-logprob.mean()``), its evaluation and the scoring of sampled tokens in one pass over
+the logits in their own type: no fp32 copy, no log-softmax tensor. GPU tensors run the HIP kernels
+(csrc/hip/hip_logprob.hip) on the current stream without synchronising; CPU tensors run plain torch operations.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from .._native import C
+from .kernels import WIRE_DTYPE, _check, hip_device_count
+
+MAX_TOP_LOGPROBS = 64
+
+
+class TokenLogprobs(NamedTuple):
+    logprob: torch.Tensor                 # fp32, logits.shape[:-1]; 0 where the target is ignore_index
+    entropy: torch.Tensor                 # fp32, logits.shape[:-1]
+    top_logprob: Optional[torch.Tensor]   # fp32, logits.shape[:-1] + (top_k,), falling; None for top_k = 0
+    top_index: Optional[torch.Tensor]     # int64, the alternatives' tokens
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def _rows(logits: torch.Tensor) -> torch.Tensor:
+    """[rows, vocab] with the vocabulary contiguous: a view where the strides allow it, else a copy."""
+    x = logits.reshape(-1, logits.shape[-1])
+    return x if x.shape[1] == 1 or x.stride(1) == 1 else x.contiguous()
+
+
+def _host_forward(x: torch.Tensor, targets: torch.Tensor, top_k: int, ignore_index: int):
+    xf = x.float()
+    m = xf.masked_fill(xf.isnan(), -torch.inf).amax(dim=1)
+    mu = torch.where(m == -torch.inf, 0.0, m)
+    d = xf - mu[:, None]
+    e = d.exp()
+    s = e.sum(dim=1)
+    empty = (m == -torch.inf) & (s == 0)
+    log_s = torch.where(empty, 0.0, s.log())
+    entropy = torch.where(empty, 0.0, log_s - (e * d.clamp(min=-200.0)).sum(dim=1) / s)
+    stats = torch.stack([m, log_s], dim=1)
+    logp = torch.where(empty[:, None], -torch.inf, (xf - m[:, None]) - log_s[:, None])
+    known = (targets >= 0) & (targets < x.shape[1])
+    lp = logp.gather(1, torch.where(known, targets, 0)[:, None])[:, 0]
+    logprob = torch.where(targets == ignore_index, 0.0, torch.where(known, lp, torch.nan))
+    top_lp = top_ix = None
+    if top_k:
+        order = xf.masked_fill(xf.isnan(), -torch.inf)
+        top_ix = order.sort(dim=1, descending=True, stable=True).indices[:, :top_k].contiguous()
+        top_lp = logp.gather(1, top_ix)
+    return logprob, entropy, stats, top_lp, top_ix
+
+
+def _host_backward(x, targets, ignore_index, entropy, stats, top_ix, g_lp, g_h, g_top):
+    m, log_s = stats[:, :1], stats[:, 1:]
+    empty = (m == -torch.inf) & (log_s == 0)
+    logp = (x.float() - m) - log_s
+    zero = torch.zeros_like(entropy)
+    used = targets != ignore_index
+    known = (targets >= 0) & (targets < x.shape[1])
+    g_lp = zero if g_lp is None else torch.where(used, g_lp, 0.0)
+    g_h = zero if g_h is None else g_h
+    gs = torch.where(used & ~known, torch.nan, g_lp) + (0.0 if g_top is None else g_top.sum(dim=1))
+    d = -logp.exp() * (gs[:, None] + g_h[:, None] * (logp.clamp(min=-200.0) + entropy[:, None]))
+    d.scatter_add_(1, torch.where(known, targets, 0)[:, None], torch.where(known, g_lp, 0.0)[:, None])
+    if g_top is not None:
+        d.scatter_add_(1, top_ix, g_top)
+    return torch.where(empty, 0.0, d).to(x.dtype)
+
+
+def _device_forward(x: torch.Tensor, targets: torch.Tensor, top_k: int, ignore_index: int):
+    n, v = x.shape
+    logprob, entropy = (torch.empty(n, dtype=torch.float32, device=x.device) for _ in range(2))
+    stats = torch.empty((n, 2), dtype=torch.float32, device=x.device)
+    top_lp = top_ix = None
+    if top_k:
+        top_lp = torch.empty((n, top_k), dtype=torch.float32, device=x.device)
+        top_ix = torch.empty((n, top_k), dtype=torch.int64, device=x.device)
+    _check(C.pcclxTokenLogprobs(x.data_ptr(), x.stride(0), n, v, WIRE_DTYPE[x.dtype], targets.data_ptr(),
+                                ignore_index, top_k, logprob.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
+                                _ptr(top_lp), _ptr(top_ix), torch.cuda.current_stream(x.device).cuda_stream),
+           "token_logprobs")
+    return logprob, entropy, stats, top_lp, top_ix
+
+
+def _device_backward(x, targets, ignore_index, entropy, stats, top_ix, g_lp, g_h, g_top):
+    n, v = x.shape
+    d = torch.empty((n, v), dtype=x.dtype, device=x.device)
+    g_lp, g_h, g_top = (None if g is None else g.contiguous() for g in (g_lp, g_h, g_top))
+    _check(C.pcclxTokenLogprobsGrad(x.data_ptr(), x.stride(0), n, v, WIRE_DTYPE[x.dtype], targets.data_ptr(),
+                                    ignore_index, 0 if top_ix is None else top_ix.shape[1], entropy.data_ptr(),
+                                    stats.data_ptr(), _ptr(top_ix), _ptr(g_lp), _ptr(g_h), _ptr(g_top), d.data_ptr(),
+                                    torch.cuda.current_stream(x.device).cuda_stream), "token_logprobs_grad")
+    return d
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, top_k, ignore_index):
+        shape = targets.shape
+        x, t = _rows(logits), targets.reshape(-1).contiguous()
+        run = _device_forward if x.is_cuda else _host_forward
+        with torch.cuda.device(x.device) if x.is_cuda else torch.no_grad():
+            logprob, entropy, stats, top_lp, top_ix = run(x, t, top_k, ignore_index)
+        logprob, entropy = logprob.view(shape), entropy.view(shape)
+        if top_k:
+            top_lp, top_ix = top_lp.view(shape + (top_k,)), top_ix.view(shape + (top_k,))
+            ctx.mark_non_differentiable(top_ix)
+        ctx.ignore_index = ignore_index
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(logits, t, entropy, stats, top_ix)
+        return logprob, entropy, top_lp, top_ix
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_lp, g_h, g_top, _):
+        logits, t, entropy, stats, top_ix = ctx.saved_tensors
+        if g_lp is None and g_h is None and g_top is None:
+            return None, None, None, None
+        x = _rows(logits)
+        flat = lambda g: None if g is None else g.reshape(-1)  # noqa: E731
+        if top_ix is not None:
+            top_ix = top_ix.reshape(len(t), -1)
+            g_top = None if g_top is None else g_top.reshape(len(t), -1)
+        run = _device_backward if x.is_cuda else _host_backward
+        with torch.cuda.device(x.device) if x.is_cuda else torch.no_grad():
+            d = run(x, t, ctx.ignore_index, entropy.reshape(-1), stats, top_ix, flat(g_lp), flat(g_h), g_top)
+        return d.view(logits.shape), None, None, None
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top_k: int = 0,
+                   ignore_index: int = -100) -> TokenLogprobs:
+    """Log probability of ``targets`` under ``softmax(logits)``, the entropy of that distribution, and its ``top_k``
+    most likely tokens.
+
+    ``logits``: fp32 / bf16 / fp16, any leading shape and strides (the vocabulary should be contiguous: other layouts
+    are copied). ``targets``: int64, ``logits.shape[:-1]``, on the same device. Results are fp32, sums in fp32; equal
+    calls give equal bits. ``top_k`` at most 64; equal logits rank by the lower index, NaN with ``-inf``.
+
+    * targets equal to ``ignore_index`` have log probability 0 and no gradient through it;
+    * a target outside the vocabulary has log probability NaN, and NaN gradients (checking it would wait for the GPU);
+    * ``-inf`` logits are masked tokens: probability 0, no share in the entropy, gradient 0;
+    * a row whose every logit is ``-inf`` has entropy 0, log probabilities ``-inf`` and gradient 0;
+    * a row with a NaN or ``+inf`` has NaN results and gradients.
+
+    ``logprob``, ``entropy`` and ``top_logprob`` are differentiable (once) with respect to ``logits``; the call and its
+    backward only queue kernels, so both may be captured into a graph.
+    """
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"token_logprobs: logits need a vocabulary dimension, got shape {tuple(logits.shape)}")
+    if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError(f"token_logprobs: logits must be fp32/bf16/fp16, got {logits.dtype}")
+    if targets.dtype != torch.int64:
+        raise TypeError(f"token_logprobs: targets must be int64, got {targets.dtype}")
+    if targets.shape != logits.shape[:-1]:
+        raise ValueError(f"token_logprobs: targets of shape {tuple(targets.shape)} do not match logits of shape "
+                         f"{tuple(logits.shape)}")
+    if targets.device != logits.device:
+        raise ValueError(f"token_logprobs: targets on {targets.device}, logits on {logits.device}")
+    if not 0 <= top_k <= min(MAX_TOP_LOGPROBS, logits.shape[-1]):
+        raise ValueError(f"token_logprobs: top_k {top_k} is not in 0..{min(MAX_TOP_LOGPROBS, logits.shape[-1])}")
+    if targets.numel() >= 1 << 31 or logits.shape[-1] >= 1 << 31:
+        raise ValueError("token_logprobs: at most 2^31 - 1 rows and tokens of vocabulary")
+    if logits.device.type == "cuda":
+        if hip_device_count() == 0:
+            raise RuntimeError("pccl-amd HIP backend (libpccl_hip.so) is not loaded but a GPU tensor was passed")
+    elif logits.device.type != "cpu":
+        raise ValueError(f"token_logprobs: no kernel for device {logits.device}")
+    return TokenLogprobs(*_TokenLogprobs.apply(logits, targets, int(top_k), int(ignore_index)))

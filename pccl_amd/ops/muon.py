@@ -1,0 +1,195 @@
+"""Newton-Schulz orthogonalisation, and the Muon optimiser step built on it.
+
+Muon replaces the momentum update U of a weight matrix by its orthogonal factor, approximated by a few steps of
+``X <- a X + (b A + c A A) X`` with ``A = X X^T`` from ``X = U / ||U||_F``; embeddings, biases and norms keep another
+optimiser (:class:`pccl_amd.parallel.Muon`). GPU tensors run the HIP kernels (csrc/hip/hip_muon.hip) on the current
+stream without synchronising: every matrix of a call, whatever its shape, goes through each stage in one launch. CPU
+tensors run plain torch operations.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from functools import lru_cache
+from typing import Optional, Sequence, Tuple
+
+import torch
+
+from .._native import C
+from .kernels import WIRE_DTYPE, _check, hip_device_count
+
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+@lru_cache(maxsize=64)
+def _check_coefficients(coefficients: Tuple[float, ...], steps: int) -> None:
+    """The kernels hold X, A and P = bA + cAA as scaled fp16 pairs (csrc/kernels/muon_common.hpp), so singular values
+    have to stay below 4 from the unit interval on, and P's eigenvalues below 12 in size."""
+    if len(coefficients) != 3:
+        raise ValueError(f"orthogonalize: three coefficients (a, b, c), got {coefficients}")
+    if not 1 <= steps <= 100:
+        raise ValueError(f"orthogonalize: steps must be in 1..100, got {steps}")
+    a, b, c = coefficients
+    top = 1.0
+    for _ in range(steps):
+        s = torch.linspace(0, top, 4097, dtype=torch.float64)
+        p = b * s ** 2 + c * s ** 4
+        size, nxt = float(p.abs().max()), float((s * (a + p)).abs().max())
+        if not (math.isfinite(size) and math.isfinite(nxt)) or size > 11.5 or nxt > 3.9:
+            raise ValueError(f"orthogonalize: coefficients {coefficients} let singular values grow out of range")
+        top = max(nxt, 1e-30)
+
+
+def _host_orthogonalize(x: torch.Tensor, steps: int, coefficients, eps: float) -> torch.Tensor:
+    a, b, c = coefficients
+    norm = x.double().square().sum(dim=(-2, -1), keepdim=True).sqrt()
+    y = (x.double() / torch.where(norm < eps, eps, norm)).float()
+    flip = y.shape[-2] > y.shape[-1]
+    y = y.mT if flip else y
+    for _ in range(steps):
+        g = y @ y.mT
+        y = a * y + (b * g + c * (g @ g)) @ y
+    return y.mT if flip else y
+
+
+def _queue(entries, gtype, wtype, mom, alpha, decay, momentum, nesterov, steps, coefficients, eps, device, what):
+    """entries: (count, rows, cols, g, w) with tensors g and w; mom: tensors or None."""
+    if hip_device_count() == 0:
+        raise RuntimeError("pccl-amd HIP backend (libpccl_hip.so) is not loaded but a GPU tensor was passed")
+    n = len(entries)
+    shapes = (ctypes.c_int64 * (3 * n))(*[v for e in entries for v in e[:3]])
+    need = C.pcclxMuonWorkspace(n, shapes)
+    if need < 0:
+        raise ValueError(f"{what}: a matrix is too large")
+    pointers = lambda ts: (ctypes.c_void_p * n)(*[t.data_ptr() for t in ts])  # noqa: E731
+    with torch.cuda.device(device):
+        work = torch.empty(need, dtype=torch.uint8, device=device)
+        rc = C.pcclxMuon(n, shapes, pointers(e[3] for e in entries), WIRE_DTYPE[gtype],
+                         pointers(e[4] for e in entries), WIRE_DTYPE[wtype], pointers(mom) if mom else None,
+                         (ctypes.c_float * n)(*alpha) if alpha else None, decay, momentum, int(nesterov), steps,
+                         (ctypes.c_float * 3)(*coefficients), eps, work.data_ptr(), need,
+                         torch.cuda.current_stream(device).cuda_stream)
+    if rc == -3:
+        raise ValueError(f"{what}: a tensor that is written shares memory with another one of the call")
+    _check(rc, what)
+
+
+def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence[float] = COEFFICIENTS,
+                  eps: float = 1e-7, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The orthogonal factor of each matrix of ``x`` ([..., m, n], fp32 / bf16 / fp16), by ``steps`` Newton-Schulz
+    steps from ``x / max(||x||_F, eps)``; singular values end near 1, in about [0.7, 1.2] with the default coefficients.
+
+    Not differentiable. The norm is summed in 64 bits; an fp32 or fp16 result has the error of fp32 products, a bf16
+    result one rounding more than bf16's own. A zero matrix gives zero, one with a NaN or an infinity gives NaN.
+    Non-contiguous input is copied. ``out`` (contiguous, of x's shape and type) may be ``x`` itself.
+    """
+    coefficients = tuple(float(v) for v in coefficients)
+    _check_coefficients(coefficients, int(steps))
+    if x.dim() < 2:
+        raise ValueError(f"orthogonalize: a matrix or a stack of them, got shape {tuple(x.shape)}")
+    if x.dtype not in _TYPES:
+        raise TypeError(f"orthogonalize: fp32/bf16/fp16, got {x.dtype}")
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise RuntimeError("orthogonalize is not differentiable: call it under no_grad or on a detached tensor")
+    if not eps > 0 or not math.isfinite(eps):
+        raise ValueError(f"orthogonalize: eps must be positive, got {eps}")
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or not out.is_contiguous():
+        raise ValueError("orthogonalize: out must be contiguous and match x in shape, type and device")
+    if x.numel() == 0:
+        return out
+    if x.device.type == "cpu":
+        return out.copy_(_host_orthogonalize(x, int(steps), coefficients, eps))
+    if x.device.type != "cuda":
+        raise ValueError(f"orthogonalize: no kernel for device {x.device}")
+    m, n = x.shape[-2:]
+    _queue([(x.numel() // (m * n), m, n, x.contiguous(), out)], x.dtype, out.dtype, None, None, 1.0, 0.0, False,
+           int(steps), coefficients, float(eps), x.device, "orthogonalize")
+    return out
+
+
+def _shape_factor(rows: int, cols: int, adjust_lr: str) -> float:
+    if adjust_lr == "original":
+        return math.sqrt(max(1.0, rows / cols))
+    if adjust_lr == "match_rms_adamw":
+        return 0.2 * math.sqrt(max(rows, cols))
+    if adjust_lr == "none":
+        return 1.0
+    raise ValueError(f"muon_step: adjust_lr must be 'original', 'match_rms_adamw' or 'none', got {adjust_lr!r}")
+
+
+def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
+              momentum_buffers: Sequence[torch.Tensor], *, lr: float, weight_decay: float = 0.1,
+              momentum: float = 0.95, nesterov: bool = True, steps: int = 5,
+              coefficients: Sequence[float] = COEFFICIENTS, eps: float = 1e-7, adjust_lr: str = "original") -> None:
+    """One Muon step on every matrix of ``params``, in place, by torch.optim.Muon's rule:
+
+        buf   = buf + (1 - momentum) (grad - buf)
+        u     = grad + momentum (buf - grad) if nesterov else buf
+        param = param (1 - lr weight_decay) - lr f(rows, cols) orthogonalize(u)
+
+    with f = sqrt(max(1, rows / cols)) ("original"), 0.2 sqrt(max(rows, cols)) ("match_rms_adamw") or 1 ("none").
+
+    ``params``: contiguous 2-D, one type of fp32 / bf16 / fp16; ``grads``: of their shapes, one type of the same three,
+    non-contiguous ones are copied; ``momentum_buffers``: contiguous fp32. All on one device, none of them sharing
+    memory with another (a parameter listed twice is refused). Equal calls give equal bits on every peer.
+    """
+    coefficients = tuple(float(v) for v in coefficients)
+    _check_coefficients(coefficients, int(steps))
+    if not len(params) == len(grads) == len(momentum_buffers):
+        raise ValueError(f"muon_step: {len(params)} parameters, {len(grads)} gradients and {len(momentum_buffers)} "
+                         "momentum buffers")
+    if not eps > 0 or not math.isfinite(eps):
+        raise ValueError(f"muon_step: eps must be positive, got {eps}")
+    if not 0.0 <= momentum <= 1.0:
+        raise ValueError(f"muon_step: momentum must be in 0..1, got {momentum}")
+    if not (math.isfinite(lr) and math.isfinite(weight_decay)):
+        raise ValueError(f"muon_step: lr {lr} and weight_decay {weight_decay} must be finite")
+    _shape_factor(1, 1, adjust_lr)
+    if not params:
+        return
+    device, wtype, gtype = params[0].device, params[0].dtype, grads[0].dtype
+    if wtype not in _TYPES or gtype not in _TYPES:
+        raise TypeError(f"muon_step: fp32/bf16/fp16 parameters and gradients, got {wtype} and {gtype}")
+    if device.type not in ("cpu", "cuda"):
+        raise ValueError(f"muon_step: no kernel for device {device}")
+    entries, moms, alpha = [], [], []
+    for p, g, b in zip(params, grads, momentum_buffers):
+        if p.dim() != 2 or p.shape != g.shape or p.shape != b.shape:
+            raise ValueError(f"muon_step: matrices of one shape, got parameter {tuple(p.shape)}, gradient "
+                             f"{tuple(g.shape)}, momentum {tuple(b.shape)}")
+        if p.dtype != wtype or g.dtype != gtype:
+            raise TypeError("muon_step: parameters, and gradients, must be of one type each")
+        if b.dtype != torch.float32:
+            raise TypeError(f"muon_step: momentum buffers must be fp32, got {b.dtype}")
+        if p.device != device or g.device != device or b.device != device:
+            raise ValueError("muon_step: every tensor must be on one device")
+        if not p.is_contiguous() or not b.is_contiguous():
+            raise ValueError("muon_step: parameters and momentum buffers must be contiguous")
+        if p.numel() == 0:
+            continue
+        entries.append((1, p.shape[0], p.shape[1], g.detach().contiguous(), p))
+        moms.append(b)
+        alpha.append(lr * _shape_factor(p.shape[0], p.shape[1], adjust_lr))
+    if not entries:
+        return
+    decay = 1.0 - lr * weight_decay
+    if device.type == "cuda":
+        _queue(entries, gtype, wtype, moms, alpha, decay, momentum, nesterov, int(steps), coefficients, float(eps),
+               device, "muon_step")
+        for p, b in zip(params, momentum_buffers):
+            torch.autograd.graph.increment_version(p)
+            torch.autograd.graph.increment_version(b)
+        return
+    with torch.no_grad():
+        written = [t for e, b in zip(entries, moms) for t in (e[4], b)]
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in written)
+        if any(x[1] > y[0] for x, y in zip(spans, spans[1:])):
+            raise ValueError("muon_step: a tensor that is written shares memory with another one of the call")
+        for (_, _, _, g, p), b, al in zip(entries, moms, alpha):
+            g = g.float()
+            b.add_(g - b, alpha=1.0 - momentum)
+            u = g + momentum * (b - g) if nesterov else b
+            p.copy_(p.float() * decay - al * _host_orthogonalize(u, int(steps), coefficients, eps))
