@@ -26,7 +26,6 @@ namespace {
 
 using half8 = _Float16 __attribute__((ext_vector_type(8)));
 using half4 = _Float16 __attribute__((ext_vector_type(4)));
-using short4v = short __attribute__((ext_vector_type(4)));
 using float16v = float __attribute__((ext_vector_type(16)));
 
 struct MuonTable {
@@ -44,11 +43,20 @@ __device__ __forceinline__ int entry_of(const MuonTable &t, int b) {
     return __builtin_amdgcn_readfirstlane(__popcll(__ballot(before)) - 1);
 }
 
-struct Planes { // one matrix in the workspace
+// One matrix in the workspace. X, A and P lie in panels of 64 bytes a row, all rows of a panel one after the other, so
+// that a tile's share of a panel is contiguous: an operand whose hi and lo parts are both multiplied has 16 columns a
+// panel, [16 hi | 16 lo]; one of which only the hi parts are has 32 columns a panel, and its lo parts a plane of their
+// own behind the first. A is of the first kind, X and P are what the call's products need.
+struct Planes {
     _Float16 *x0, *x1, *a, *p;
     double *part;
-    size_t xs, as; // hi -> lo distance
+    size_t xs, as; // elements of X, of A
 };
+template<bool PAIRS>
+__device__ __forceinline__ size_t panel_at(int rows, int r, int c) { // of the hi part
+    return PAIRS ? (static_cast<size_t>(c >> 4) * rows + r) * 32 + (c & 15)
+                 : (static_cast<size_t>(c >> 5) * rows + r) * 32 + (c & 31);
+}
 __device__ __forceinline__ Planes planes_of(uint8_t *ws, const MuonEntry &e, int which) {
     Planes q;
     q.xs = static_cast<size_t>(e.mp) * e.np;
@@ -78,19 +86,11 @@ struct Elem<DType::F16> {
     using S = _Float16;
 };
 
-__device__ __forceinline__ float load_as(const void *p, size_t i, DType t) {
-    if (t == DType::F32) return static_cast<const float *>(p)[i];
-    if (t == DType::BF16) return static_cast<float>(static_cast<const __bf16 *>(p)[i]);
-    return static_cast<float>(static_cast<const _Float16 *>(p)[i]);
-}
-__device__ __forceinline__ void store_as(void *p, size_t i, DType t, float v) {
-    if (t == DType::F32)
-        static_cast<float *>(p)[i] = v;
-    else if (t == DType::BF16)
-        static_cast<__bf16 *>(p)[i] = static_cast<__bf16>(v);
-    else
-        static_cast<_Float16 *>(p)[i] = static_cast<_Float16>(v);
-}
+// neighbouring elements at any element alignment (parameters are often views into one flat buffer)
+template<typename S, int N>
+struct __attribute__((packed, aligned(sizeof(S)))) Run {
+    S v[N];
+};
 
 // sum over a workgroup of 256 in a fixed order, the same in every thread
 __device__ __forceinline__ double block_sum(double v) {
@@ -122,22 +122,46 @@ __global__ __launch_bounds__(256) void k_muon_momentum(MuonTable t, MuonParams p
     const size_t per = (elems + e.partials - 1) / e.partials;
     const size_t s0 = per * part, s1 = s0 + per < elems ? s0 + per : elems;
     double sum = 0.0;
-    for (size_t k = s0 + threadIdx.x; k < s1; k += 256) {
-        float u = static_cast<float>(g[k]);
+    const auto one = [&](S gv, float &mv) {
+        float u = static_cast<float>(gv);
         if (m) {
-            const float old = m[k];
-            const float now = old + (1.0f - p.momentum) * (u - old);
-            m[k] = now;
-            u = update_of(u, now, p);
+            mv = mv + (1.0f - p.momentum) * (u - mv);
+            u = update_of(u, mv, p);
         }
         sum += static_cast<double>(u) * u;
+    };
+    size_t k = s0 + threadIdx.x * 4;
+    for (; k + 3 * 1024 + 4 <= s1; k += 4 * 1024) { // 4 x 4 elements in flight
+        Run<S, 4> gv[4];
+        Run<float, 4> mv[4] = {};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            gv[j] = *reinterpret_cast<const Run<S, 4> *>(g + k + j * 1024);
+            if (m) mv[j] = *reinterpret_cast<const Run<float, 4> *>(m + k + j * 1024);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                float v = mv[j].v[x];
+                one(gv[j].v[x], v);
+                mv[j].v[x] = v;
+            }
+            if (m) *reinterpret_cast<Run<float, 4> *>(m + k + j * 1024) = mv[j];
+        }
     }
+    for (; k < s1; k += 1024)
+        for (size_t j = k; j < k + 4 && j < s1; ++j) {
+            float v = m ? m[j] : 0.0f;
+            one(g[j], v);
+            if (m) m[j] = v;
+        }
     sum = block_sum(sum);
     if (threadIdx.x == 0) planes_of(t.ws, e, which).part[part] = sum;
 }
 
 // X_0 = U scale / max(||U||, eps) in two fp16 parts, 64 x 64 tiles; a tall U is transposed through LDS.
-template<DType G>
+template<DType G, bool PAIRS>
 __global__ __launch_bounds__(256) void k_muon_start(MuonTable t, MuonParams p) {
     using S = typename Elem<G>::S;
     __shared__ float tile[64][65];
@@ -160,15 +184,28 @@ __global__ __launch_bounds__(256) void k_muon_start(MuonTable t, MuonParams p) {
     const int ur = (flip ? n0 : m0) + r, uc = (flip ? m0 : n0) + c;
     float v[16];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-        float u = 0.0f;
-        if (ur < e.rows && uc + k < e.cols) {
-            const size_t at = static_cast<size_t>(ur) * e.cols + uc + k;
-            u = static_cast<float>(g[at]);
-            if (mom) u = update_of(u, mom[at], p);
-            u = static_cast<float>(u * scale);
+    for (int k = 0; k < 16; k += 4) {
+        const size_t at = static_cast<size_t>(ur) * e.cols + uc + k;
+        float u[4] = {}, b[4] = {};
+        if (ur < e.rows && uc + k + 4 <= e.cols) {
+            const Run<S, 4> gv = *reinterpret_cast<const Run<S, 4> *>(g + at);
+            Run<float, 4> mv = {};
+            if (mom) mv = *reinterpret_cast<const Run<float, 4> *>(mom + at);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                u[j] = static_cast<float>(gv.v[j]);
+                b[j] = mv.v[j];
+            }
+        } else if (ur < e.rows) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (uc + k + j < e.cols) {
+                    u[j] = static_cast<float>(g[at + j]);
+                    if (mom) b[j] = mom[at + j];
+                }
         }
-        v[k] = u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[k + j] = static_cast<float>((mom ? update_of(u[j], b[j], p) : u[j]) * scale);
     }
     if (flip) {
 #pragma unroll
@@ -184,144 +221,211 @@ __global__ __launch_bounds__(256) void k_muon_start(MuonTable t, MuonParams p) {
         hi[k / 8][k % 8] = h;
         lo[k / 8][k % 8] = static_cast<_Float16>(v[k] - static_cast<float>(h));
     }
-    _Float16 *x = q.x0 + static_cast<size_t>(m0 + r) * e.np + n0 + c;
-    half8 *xh = reinterpret_cast<half8 *>(x), *xl = reinterpret_cast<half8 *>(x + q.xs);
+    _Float16 *x = q.x0 + panel_at<PAIRS>(e.mp, m0 + r, n0 + c);
+    half8 *xh = reinterpret_cast<half8 *>(x), *xl = reinterpret_cast<half8 *>(x + (PAIRS ? 16 : q.xs));
     xh[0] = hi[0];
     xh[1] = hi[1];
     xl[0] = lo[0];
     xl[1] = lo[1];
 }
 
-enum { kGram = 0, kPoly = 1, kApply = 2 };
+enum { kGram = 0, kPoly = 1, kApply = 2, kFinal = 3 };
 
 struct MuonStage {
-    int cur;       // which X is read
-    int full;      // P needs its lo part
-    int last;      // the step's result goes to the caller
-    DType wt;
+    int cur; // which X is read
     float a, b, c, decay;
 };
 
-// One product stage. A workgroup computes BM x BN of it: the M side's rows (of X, A or P) lie along the sum in memory
-// and so do the N side's of kGram and kPoly, which multiply by a transpose; kApply's N side is X itself, whose
-// fragments are transposed on their way out of LDS. Both sides travel straight to LDS, 128 bytes a row: 64 of the sum,
-// or 32 with both parts. Rows are swizzled so that a fragment's 16-byte reads spread over the banks.
-// The MFMA's first operand is the N side: a lane then holds 4 neighbouring columns of one row.
-template<int KIND, int BM, int BN, bool SPLIT>
+constexpr int kStages = 3; // tiles of the sum in LDS: one is multiplied, two are on their way
+
+template<int N>
+__device__ __forceinline__ void wait_loads() { // all but the N newest loads of this wave have landed, its LDS reads too
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
+// orders LDS accesses between the lanes of one wave
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
+__device__ __forceinline__ void split_fp16(float v, _Float16 &h, _Float16 &l) {
+    h = static_cast<_Float16>(v);
+    l = static_cast<_Float16>(v - static_cast<float>(h));
+}
+
+__device__ __forceinline__ uint32_t lds_offset(const uint8_t *p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) uint8_t *)p));
+}
+
+// N-side fragments of kApply: at[z][s] is where this lane's part of the 4 x 16 block z of piece s lies, column block 1
+// lies YSTEP bytes further. In assembly, with its own wait: the builtin makes the compiler wait for the tiles that are
+// still on their way.
+template<int NT, int YSTEP>
+__device__ __forceinline__ void read_transposed(uint32_t base, const uint32_t (&at)[2][2], half8 (&f)[NT][2]) {
+    half4 h[NT][2][2];
+    if constexpr (NT == 1) {
+        asm volatile("ds_read_b64_tr_b16 %0, %4\n"
+                     "ds_read_b64_tr_b16 %1, %5\n"
+                     "ds_read_b64_tr_b16 %2, %6\n"
+                     "ds_read_b64_tr_b16 %3, %7\n"
+                     "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(h[0][0][0]), "=&v"(h[0][0][1]), "=&v"(h[0][1][0]), "=&v"(h[0][1][1])
+                     : "v"(base + at[0][0]), "v"(base + at[0][1]), "v"(base + at[1][0]), "v"(base + at[1][1])
+                     : "memory");
+    } else {
+        static_assert(NT == 2);
+        asm volatile("ds_read_b64_tr_b16 %0, %8\n"
+                     "ds_read_b64_tr_b16 %1, %9\n"
+                     "ds_read_b64_tr_b16 %2, %10\n"
+                     "ds_read_b64_tr_b16 %3, %11\n"
+                     "ds_read_b64_tr_b16 %4, %8 offset:%12\n"
+                     "ds_read_b64_tr_b16 %5, %9 offset:%12\n"
+                     "ds_read_b64_tr_b16 %6, %10 offset:%12\n"
+                     "ds_read_b64_tr_b16 %7, %11 offset:%12\n"
+                     "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(h[0][0][0]), "=&v"(h[0][0][1]), "=&v"(h[0][1][0]), "=&v"(h[0][1][1]), "=&v"(h[1][0][0]),
+                       "=&v"(h[1][0][1]), "=&v"(h[1][1][0]), "=&v"(h[1][1][1])
+                     : "v"(base + at[0][0]), "v"(base + at[0][1]), "v"(base + at[1][0]), "v"(base + at[1][1]), "n"(YSTEP)
+                     : "memory");
+    }
+#pragma unroll
+    for (int y = 0; y < NT; ++y)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) f[y][s] = __builtin_shufflevector(h[y][0][s], h[y][1][s], 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// 16-byte pieces of a panel's 64-byte rows trade places in LDS by the row: a fragment's reads (one piece of 8 rows, or
+// two of 4) then meet no bank twice
+__device__ __forceinline__ int swizzle(int r) { return (r & 2) | ((r >> 2) & 1); }
+
+// One product stage. A workgroup computes BM x BN of it. The M side's rows (of X, A or P) lie along the sum, and so do
+// the N side's of kGram and kPoly, which multiply by a transpose; kApply's and kFinal's N side is X itself, whose
+// fragments are transposed on their way out of LDS. Both sides travel straight to LDS, a panel of the sum at a time.
+// SPLIT: three products of the parts. PAIRS: X and P lie in pairs. The MFMA's first operand is the N side: a lane then
+// holds 4 neighbouring columns of one row.
+template<int KIND, int BM, int BN, bool SPLIT, bool PAIRS, DType W>
 __global__ __launch_bounds__(256, 2) void k_muon_product(MuonTable t, MuonStage st) {
     constexpr int WM = BM / 2, WN = BN / 2, MT = WM / 32, NT = WN / 32;
-    constexpr int BK = SPLIT ? 32 : 64;
-    constexpr bool NN = KIND == kApply;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2][(BM + BN) * 128];
+    constexpr int BK = SPLIT ? 16 : 32; // columns of a panel, the step along the sum
+    constexpr bool NN = KIND == kApply || KIND == kFinal;
+    constexpr int kTile = (BM + BN) * 64;
+    constexpr int kSlice = 32 * (WN + 4) * 4; // 32 rows of a wave's results, padded against bank conflicts
+    constexpr int kLds = kStages * kTile > 4 * kSlice ? kStages * kTile : 4 * kSlice;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
 
     const int per_xcd = gridDim.x / 8; // workgroups of one matrix next to each other on one chiplet's L2
     const int blk = static_cast<int>(blockIdx.x) < per_xcd * 8 ? (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3)
                                                                  : static_cast<int>(blockIdx.x);
     const int i = entry_of(t, blk);
     const MuonEntry &e = t.e[i];
-    const int tm = (e.mp + BM - 1) / BM, tn = NN ? (e.np + BN - 1) / BN : tm;
-    const int tiles = NN ? tm * tn : tm * (tm + 1) / 2;
-    const int b = blk - t.first[i], which = b / tiles;
-    int ti, tj;
+    const int rows = e.mp;
+    const int tm = (rows + BM - 1) / BM, tn = ((NN ? e.np : rows) + BN - 1) / BN;
+    int ti, tj, which;
     if constexpr (NN) {
-        ti = b % tiles % tm;
-        tj = b % tiles / tm;
-    } else { // tiles on and above the diagonal
+        const int b = blk - t.first[i];
+        which = b / (tm * tn);
+        ti = b % (tm * tn) % tm;
+        tj = b % (tm * tn) / tm;
+    } else { // tiles that reach the diagonal or lie above it
+        constexpr int R = BM / BN;
+        const int tiles = tm * tn - R * (tm * (tm - 1) / 2);
+        const int b = blk - t.first[i];
+        which = b / tiles;
         int rest = b % tiles;
         ti = 0;
-        while (rest >= tm - ti) rest -= tm - ti++;
-        tj = ti + rest;
+        while (rest >= tn - R * ti) rest -= tn - R * ti++;
+        tj = R * ti + rest;
     }
     const Planes q = planes_of(t.ws, e, which);
     const _Float16 *x = st.cur ? q.x1 : q.x0;
-    _Float16 *xn = st.cur ? q.x0 : q.x1;
     const int m0 = ti * BM, n0 = tj * BN;
-    const int K = KIND == kGram ? e.np : e.mp;
+    const int K = KIND == kGram ? e.np : rows;
     const _Float16 *ms = KIND == kGram ? x : KIND == kPoly ? q.a : q.p;
     const _Float16 *ns = KIND == kPoly ? q.a : x;
-    const size_t mps = KIND == kGram ? q.xs : q.as, nps = KIND == kPoly ? q.as : q.xs;
-    const int mld = K, nld = NN ? e.np : K;
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    // source of each 16-byte piece this lane brings to LDS; rows and columns past the matrix repeat its last ones
-    constexpr int MI = BM / 32, NI = BN / 32;
+    // source of each 16-byte piece this lane brings to LDS; rows and panels past the matrix repeat its last ones
+    constexpr int MI = BM / 64, NI = BN / 64;
     const _Float16 *mp[MI], *np[NI];
+    const int lrow = lane >> 2;
+    const int lpiece = ((lane & 3) ^ swizzle(lrow)) * 8;
 #pragma unroll
     for (int k = 0; k < MI; ++k) {
-        const int r = (wave * MI + k) * 8 + (lane >> 3), c = (lane & 7) ^ (r & 7);
-        const int gr = m0 + r < e.mp ? m0 + r : e.mp - 1;
-        mp[k] = ms + (SPLIT ? (c >> 2) * mps + (c & 3) * 8 : c * 8) + static_cast<size_t>(gr) * mld;
+        const int r = m0 + (wave * MI + k) * 16 + lrow;
+        mp[k] = ms + static_cast<size_t>(r < rows ? r : rows - 1) * 32 + lpiece;
     }
-    constexpr int LPR = BN / 8; // lanes per row of the N side of kApply
-    constexpr int SWZ = BN == 128 ? 2 : 1;
 #pragma unroll
     for (int k = 0; k < NI; ++k) {
-        if constexpr (NN) {
-            const int r = (wave * NI + k) * (64 / LPR) + lane / LPR, c = (lane % LPR) ^ ((r & 3) << SWZ);
-            const int gc = n0 + c * 8 < e.np ? n0 + c * 8 : e.np - 8;
-            np[k] = ns + (SPLIT ? (r >> 5) * nps + static_cast<size_t>(r & 31) * nld : static_cast<size_t>(r) * nld) + gc;
+        if constexpr (NN) { // BK rows of BN / BK panels
+            const int j = wave * NI + k, panels = e.np / BK;
+            const int pn = n0 / BK + j / (BK / 16);
+            np[k] = ns + (static_cast<size_t>(pn < panels ? pn : panels - 1) * rows + j % (BK / 16) * 16 + lrow) * 32 + lpiece;
         } else {
-            const int r = (wave * NI + k) * 8 + (lane >> 3), c = (lane & 7) ^ (r & 7);
-            const int gr = n0 + r < e.mp ? n0 + r : e.mp - 1;
-            np[k] = ns + (SPLIT ? (c >> 2) * nps + (c & 3) * 8 : c * 8) + static_cast<size_t>(gr) * nld;
+            const int r = n0 + (wave * NI + k) * 16 + lrow;
+            np[k] = ns + static_cast<size_t>(r < rows ? r : rows - 1) * 32 + lpiece;
         }
     }
-    const size_t nstep = NN ? static_cast<size_t>(BK) * nld : BK;
+    const size_t mstep = static_cast<size_t>(rows) * 32, nstep = NN ? BK * 32 : mstep;
     const auto fetch = [&](int buf) {
-        uint8_t *to = lds[buf];
+        uint8_t *to = lds + buf * kTile;
 #pragma unroll
         for (int k = 0; k < MI; ++k) {
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)mp[k],
                                              (__attribute__((address_space(3))) void *)(to + (wave * MI + k) * 1024), 16,
                                              0, 0);
-            mp[k] += BK;
+            mp[k] += mstep;
         }
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
             __builtin_amdgcn_global_load_lds(
                 (const __attribute__((address_space(1))) void *)np[k],
-                (__attribute__((address_space(3))) void *)(to + BM * 128 + (wave * NI + k) * 1024), 16, 0, 0);
+                (__attribute__((address_space(3))) void *)(to + BM * 64 + (wave * NI + k) * 1024), 16, 0, 0);
             np[k] += nstep;
         }
     };
 
     const int wm = (wave & 1) * WM, wn = (wave >> 1) * WN;
     const int half = lane >> 5, l32 = lane & 31;
-    float16v acc[NT][MT] = {};
-    fetch(0);
-    for (int k0 = 0, buf = 0; k0 < K; k0 += BK, buf ^= 1) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads(); // the tile has landed, and the other buffer's readers are done
-        const uint8_t *ml = lds[buf], *nl = lds[buf] + BM * 128;
-        half8 mf[MT][4], nf[NT][4]; // four pieces of 16 of the sum: hi 0, 1 and lo 0, 1, or 0..3
+    uint32_t tr[2][2] = {}; // transposed reads: 16 lanes fetch a 4 x 16 block of X and get its columns, 4 of the sum each
+    if constexpr (NN) {
+        const int l16 = lane & 15, cb = (lane >> 4) & 1;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
+        for (int z = 0; z < 2; ++z)
 #pragma unroll
-            for (int u = 0; u < MT; ++u) {
-                const int r = wm + u * 32 + l32;
-                mf[u][s] = *reinterpret_cast<const half8 *>(ml + r * 128 + (((2 * s + half) ^ (r & 7)) << 4));
+            for (int s = 0; s < 2; ++s) {
+                const int r = 8 * half + 4 * z + (l16 >> 2) + (SPLIT ? 0 : 16 * s);
+                const int piece = (SPLIT ? 2 * s : 2 * cb) + ((l16 & 3) >> 1);
+                const int panel = SPLIT ? wn / 16 + cb : wn / 32;
+                tr[z][s] = panel * (BK * 64) + r * 64 + ((piece ^ swizzle(r)) << 4) + (l16 & 1) * 8;
             }
+    }
+    float16v acc[NT][MT] = {};
+    const int steps = K / BK; // K is a multiple of 64
+    fetch(0);
+    fetch(1);
+    for (int k = 0, buf = 0; k < steps; ++k) {
+        if (k + 1 < steps)
+            wait_loads<MI + NI>();
+        else
+            wait_loads<0>();
+        __builtin_amdgcn_s_barrier(); // tile k has landed for every wave, and all are done with tile k - 1
+        asm volatile("" ::: "memory");
+        const uint8_t *ml = lds + buf * kTile, *nl = ml + BM * 64;
+        half8 mf[MT][2], nf[NT][2]; // two pieces of 16 of the sum: hi and lo of one, or both of 32
 #pragma unroll
-            for (int y = 0; y < NT; ++y) {
-                if constexpr (NN) {
-                    const int l16 = lane & 15;
-                    const int col = wn + y * 32 + ((lane >> 4) & 1) * 16 + (l16 & 3) * 4;
-                    half4 h[2];
+        for (int s = 0; s < 2; ++s) {
+            const int at = l32 * 64 + (((2 * s + half) ^ swizzle(l32)) << 4);
 #pragma unroll
-                    for (int z = 0; z < 2; ++z) {
-                        const int r = 16 * s + 8 * half + 4 * z + (l16 >> 2);
-                        const uint8_t *at = nl + r * (BN * 2) + (((col >> 3) ^ ((r & 3) << SWZ)) << 4) + (col & 7) * 2;
-                        h[z] = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                             (__attribute__((address_space(3))) short4v *)at));
-                    }
-                    nf[y][s] = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
-                } else {
-                    const int r = wn + y * 32 + l32;
-                    nf[y][s] = *reinterpret_cast<const half8 *>(nl + r * 128 + (((2 * s + half) ^ (r & 7)) << 4));
-                }
+            for (int u = 0; u < MT; ++u) mf[u][s] = *reinterpret_cast<const half8 *>(ml + (wm + u * 32) * 64 + at);
+            if constexpr (!NN) {
+#pragma unroll
+                for (int y = 0; y < NT; ++y) nf[y][s] = *reinterpret_cast<const half8 *>(nl + (wn + y * 32) * 64 + at);
             }
         }
-        if (k0 + BK < K) fetch(buf ^ 1);
+        if constexpr (NN) read_transposed<NT, 32 / BK * BK * 64>(lds_offset(nl), tr, nf);
+        buf = buf == kStages - 1 ? 0 : buf + 1;
+        if (k + 2 < steps) fetch(buf == kStages - 1 ? 0 : buf + 1); // over tile k - 1
         const auto mul = [&](int sn, int sm) {
 #pragma unroll
             for (int y = 0; y < NT; ++y)
@@ -329,104 +433,164 @@ __global__ __launch_bounds__(256, 2) void k_muon_product(MuonTable t, MuonStage 
                 for (int u = 0; u < MT; ++u)
                     acc[y][u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(nf[y][sn], mf[u][sm], acc[y][u], 0, 0, 0);
         };
+        mul(0, 0);
         if constexpr (SPLIT) {
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                mul(s, s);
-                mul(s, s + 2);
-                mul(s + 2, s);
-            }
+            mul(0, 1);
+            mul(1, 0);
         } else {
-#pragma unroll
-            for (int s = 0; s < 4; ++s) mul(s, s);
+            mul(1, 1);
         }
     }
+    __syncthreads(); // the tiles' memory now carries results
 
-    const auto split = [](float v, _Float16 &h, _Float16 &l) {
-        h = static_cast<_Float16>(v);
-        l = static_cast<_Float16>(v - static_cast<float>(h));
-    };
+    // Results leave through LDS, 32 rows of a wave at a time: a lane then has 8 neighbouring columns of a row. What it
+    // needs from memory is asked for before.
     const bool flip = e.rows > e.cols;
     const int small = flip ? e.cols : e.rows, large = flip ? e.rows : e.cols;
+    const int nmax = NN ? e.np : rows;
+    constexpr int LR = WN / 8, O = 32 / (64 / LR); // lanes of a row, and pieces of a slice
+    constexpr int kPitch = WN + 4;
+    float *slice = reinterpret_cast<float *>(lds + wave * kSlice);
+    using WS = typename Elem<W>::S;
+    WS *w = KIND == kFinal ? static_cast<WS *>(e.w) + static_cast<size_t>(e.rows) * e.cols * which : nullptr;
+    const float alpha = e.alpha;
+    const bool step = e.mom != nullptr;
+    const auto final_value = [&](float v, WS old) {
+        v *= 1.0f / kMuonScaleX;
+        return static_cast<WS>(step ? static_cast<float>(old) * st.decay - alpha * v : v);
+    };
+    constexpr bool kInPairs = NN ? PAIRS : true;  // layout of what the epilogue reads (X, or A)
+    constexpr bool kOutPairs = KIND == kGram || PAIRS; // and writes (A, P or X)
+    const size_t in_lo = kInPairs ? 16 : q.xs, out_lo = kOutPairs ? 16 : q.xs;
+    const _Float16 *in = NN ? x : q.a;
+    _Float16 *out = KIND == kGram ? q.a : KIND == kPoly ? q.p : st.cur ? q.x0 : q.x1;
+    const bool lows = KIND != kPoly || PAIRS; // P's lo parts are only there to be multiplied
 #pragma unroll
-    for (int y = 0; y < NT; ++y) {
+    for (int u = 0; u < MT; ++u) {
+        const int mb = m0 + wm + u * 32;
+        half8 ih[O], il[O];
+        if constexpr (KIND != kGram) {
 #pragma unroll
-        for (int u = 0; u < MT; ++u) {
-            const int mb = m0 + wm + u * 32, nb = n0 + wn + y * 32;
-            if (mb >= e.mp || nb >= (NN ? e.np : e.mp)) continue;
-            const int m = mb + l32;
+            for (int o = 0; o < O; ++o) {
+                const int m = mb + o * (64 / LR) + lane / LR, n = n0 + wn + lane % LR * 8;
+                if (m < rows && n < nmax) {
+                    const size_t at = panel_at<kInPairs>(rows, m, n);
+                    ih[o] = *reinterpret_cast<const half8 *>(in + at);
+                    il[o] = *reinterpret_cast<const half8 *>(in + at + in_lo);
+                }
+            }
+        }
+#pragma unroll
+        for (int y = 0; y < NT; ++y)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const int n = nb + 8 * k + 4 * half;
+                float4 v;
+                v.x = acc[y][u][4 * k];
+                v.y = acc[y][u][4 * k + 1];
+                v.z = acc[y][u][4 * k + 2];
+                v.w = acc[y][u][4 * k + 3];
+                *reinterpret_cast<float4 *>(slice + l32 * kPitch + y * 32 + 8 * k + 4 * half) = v;
+            }
+        wave_sync();
+#pragma unroll
+        for (int o = 0; o < O; ++o) {
+            const int r = o * (64 / LR) + lane / LR, c = lane % LR * 8;
+            const int m = mb + r, n = n0 + wn + c;
+            if (m >= rows || n >= nmax) continue;
+            float v[8];
+            *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(slice + r * kPitch + c);
+            *reinterpret_cast<float4 *>(v + 4) = *reinterpret_cast<const float4 *>(slice + r * kPitch + c + 4);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if constexpr (KIND == kGram) {
+                    v[k] *= kMuonScaleA / (kMuonScaleX * kMuonScaleX);
+                } else {
+                    const float old = static_cast<float>(ih[o][k]) + static_cast<float>(il[o][k]);
+                    if constexpr (NN)
+                        v[k] = v[k] * (1.0f / kMuonScaleP) + st.a * old;
+                    else
+                        v[k] = v[k] * (st.c * (kMuonScaleP / (kMuonScaleA * kMuonScaleA))) +
+                               (st.b * (kMuonScaleP / kMuonScaleA)) * old;
+                }
+            }
+            if constexpr (KIND != kFinal) {
+                half8 oh, ol;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    _Float16 h, l;
+                    split_fp16(v[k], h, l);
+                    oh[k] = h;
+                    ol[k] = l;
+                }
+                const size_t at = panel_at<kOutPairs>(rows, m, n);
+                *reinterpret_cast<half8 *>(out + at) = oh;
+                if (lows) *reinterpret_cast<half8 *>(out + at + out_lo) = ol;
+            }
+            if (KIND != kApply) { // read again, along the columns or by other lanes
+                *reinterpret_cast<float4 *>(slice + r * kPitch + c) = *reinterpret_cast<float4 *>(v);
+                *reinterpret_cast<float4 *>(slice + r * kPitch + c + 4) = *reinterpret_cast<float4 *>(v + 4);
+            }
+        }
+        wave_sync();
+        if constexpr (!NN) {
+            // the mirrored half, of tiles behind the diagonal's: 8 of the 32 rows of one column per lane
+            if (tj >= (ti + 1) * (BM / BN) && mb < rows) {
+#pragma unroll
+                for (int o = 0; o < WN; o += 16) {
+                    const int c = o + (lane >> 2), r = (lane & 3) * 8;
+                    const int n = n0 + wn + c;
+                    if (n >= rows) continue;
+                    half8 oh, ol;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        _Float16 h, l;
+                        split_fp16(slice[(r + k) * kPitch + c], h, l);
+                        oh[k] = h;
+                        ol[k] = l;
+                    }
+                    const size_t at = panel_at<kOutPairs>(rows, n, mb + r);
+                    *reinterpret_cast<half8 *>(out + at) = oh;
+                    if (lows) *reinterpret_cast<half8 *>(out + at + out_lo) = ol;
+                }
+            }
+        }
+        if constexpr (KIND == kFinal) {
+            // the caller's matrix: its rows lie along n, or along m where it was transposed; 4 elements per lane
+            constexpr int P = WN * 32 / 256; // pieces of a slice
+            const int lr = flip ? lane >> 3 : lane / (WN / 4), lc = flip ? (lane & 7) * 4 : lane % (WN / 4) * 4;
+            Run<WS, 4> old[P];
+            bool whole[P];
+            size_t at[P];
+#pragma unroll
+            for (int k = 0; k < P; ++k) { // rows of the caller's: n = lr + 8 k, or m = lr + (256 / WN) k
+                const int m = flip ? mb + lc : mb + lr + 256 / WN * k;
+                const int n = flip ? n0 + wn + lr + 8 * k : n0 + wn + lc;
+                at[k] = flip ? static_cast<size_t>(n) * e.cols + m : static_cast<size_t>(m) * e.cols + n;
+                whole[k] = flip ? n < large && m + 4 <= small : m < small && n + 4 <= large;
+                if (whole[k] && step) old[k] = *reinterpret_cast<const Run<WS, 4> *>(w + at[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
                 float v[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = acc[y][u][4 * k + r];
-                if constexpr (KIND == kApply) {
-                    const size_t at = static_cast<size_t>(m) * e.np + n;
-                    const half4 xh = *reinterpret_cast<const half4 *>(x + at);
-                    const half4 xl = *reinterpret_cast<const half4 *>(x + q.xs + at);
-                    half4 oh, ol;
+                for (int j = 0; j < 4; ++j)
+                    v[j] = flip ? slice[(lc + j) * kPitch + lr + 8 * k] : slice[(lr + 256 / WN * k) * kPitch + lc + j];
+                if (whole[k]) {
+                    Run<WS, 4> now;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        v[r] = v[r] * (1.0f / kMuonScaleP) +
-                               st.a * (static_cast<float>(xh[r]) + static_cast<float>(xl[r]));
-                        _Float16 h, l;
-                        split(v[r], h, l);
-                        oh[r] = h;
-                        ol[r] = l;
-                    }
-                    if (!st.last) {
-                        *reinterpret_cast<half4 *>(xn + at) = oh;
-                        *reinterpret_cast<half4 *>(xn + q.xs + at) = ol;
-                    } else {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            if (m >= small || n + r >= large) continue;
-                            const size_t o = static_cast<size_t>(e.rows) * e.cols * which +
-                                             (flip ? static_cast<size_t>(n + r) * e.cols + m
-                                                   : static_cast<size_t>(m) * e.cols + n + r);
-                            float out = v[r] * (1.0f / kMuonScaleX);
-                            if (e.mom) out = load_as(e.w, o, st.wt) * st.decay - e.alpha * out;
-                            store_as(e.w, o, st.wt, out);
-                        }
-                    }
+                    for (int j = 0; j < 4; ++j) now.v[j] = final_value(v[j], old[k].v[j]);
+                    *reinterpret_cast<Run<WS, 4> *>(w + at[k]) = now;
                 } else {
-                    const size_t at = static_cast<size_t>(m) * e.mp + n;
-                    _Float16 *to = KIND == kGram ? q.a : q.p;
-                    half4 oh, ol;
-                    if constexpr (KIND == kGram) {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) v[r] *= kMuonScaleA / (kMuonScaleX * kMuonScaleX);
-                    } else {
-                        const half4 ah = *reinterpret_cast<const half4 *>(q.a + at);
-                        const half4 al = *reinterpret_cast<const half4 *>(q.a + q.as + at);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            v[r] = v[r] * (st.c * (kMuonScaleP / (kMuonScaleA * kMuonScaleA))) +
-                                   (st.b * (kMuonScaleP / kMuonScaleA)) *
-                                       (static_cast<float>(ah[r]) + static_cast<float>(al[r]));
-                    }
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        _Float16 h, l;
-                        split(v[r], h, l);
-                        oh[r] = h;
-                        ol[r] = l;
-                    }
-                    const bool lows = KIND == kGram || st.full;
-                    *reinterpret_cast<half4 *>(to + at) = oh;
-                    if (lows) *reinterpret_cast<half4 *>(to + q.as + at) = ol;
-                    if (ti != tj) {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const size_t mt = static_cast<size_t>(n + r) * e.mp + m;
-                            to[mt] = oh[r];
-                            if (lows) to[q.as + mt] = ol[r];
-                        }
+                    for (int j = 0; j < 4; ++j) {
+                        const int m = flip ? mb + lc + j : mb + lr + 256 / WN * k;
+                        const int n = flip ? n0 + wn + lr + 8 * k : n0 + wn + lc + j;
+                        if (m < small && n < large) w[at[k] + j] = final_value(v[j], step ? w[at[k] + j] : WS{});
                     }
                 }
             }
         }
+        wave_sync();
     }
 }
 
@@ -443,31 +607,32 @@ int64_t layout(MuonTable &t, F &&blocks) {
     return n;
 }
 
-template<int KIND, int BM, int BN>
-bool launch_product(MuonTable &t, const MuonStage &st, bool split, hipStream_t s) {
-    const int64_t n = layout(t, [](const MuonEntry &e) {
-        const int64_t tm = (e.mp + BM - 1) / BM;
-        return KIND == kApply ? tm * ((e.np + BN - 1) / BN) : tm * (tm + 1) / 2;
-    });
-    if (n > INT32_MAX) return false;
-    const dim3 grid(static_cast<unsigned>(n));
-    return launch_ok([&] {
-        if (split)
-            k_muon_product<KIND, BM, BN, true><<<grid, 256, 0, s>>>(t, st);
-        else if constexpr (KIND != kPoly)
-            k_muon_product<KIND, BM, BN, false><<<grid, 256, 0, s>>>(t, st);
-    });
+// tiles of one matrix in a product stage
+template<int BM, int BN>
+int64_t product_tiles(int kind, const MuonEntry &e) {
+    const int64_t tm = (e.mp + BM - 1) / BM;
+    if (kind == kApply || kind == kFinal) return tm * ((e.np + BN - 1) / BN);
+    return tm * ((e.mp + BN - 1) / BN) - BM / BN * (tm * (tm - 1) / 2);
 }
 
-template<int KIND>
-bool launch_stage(MuonTable &t, const MuonStage &st, bool split, hipStream_t s) {
-    int64_t big = 0;
+template<int KIND, int BM, int BN, bool SPLIT, bool PAIRS, DType W>
+bool launch_product(MuonTable &t, const MuonStage &st, hipStream_t s) {
+    const int64_t n = layout(t, [](const MuonEntry &e) { return product_tiles<BM, BN>(KIND, e); });
+    if (n > INT32_MAX) return false;
+    return launch_ok(
+        [&] { k_muon_product<KIND, BM, BN, SPLIT, PAIRS, W><<<dim3(static_cast<unsigned>(n)), 256, 0, s>>>(t, st); });
+}
+
+template<int KIND, bool SPLIT, bool PAIRS, DType W = DType::F32>
+bool launch_stage(MuonTable &t, const MuonStage &st, hipStream_t s) {
+    int64_t large = 0, mid = 0;
     for (int i = 0; i < t.n; ++i) {
-        const int64_t tm = (t.e[i].mp + 127) / 128;
-        big += t.e[i].count * (KIND == kApply ? tm * ((t.e[i].np + 127) / 128) : tm * (tm + 1) / 2);
+        large += t.e[i].count * product_tiles<256, 128>(KIND, t.e[i]);
+        mid += t.e[i].count * product_tiles<128, 128>(KIND, t.e[i]);
     }
-    if (big >= 256) return launch_product<KIND, 128, 128>(t, st, split, s);
-    return launch_product<KIND, 64, 64>(t, st, split, s);
+    if (large >= 256) return launch_product<KIND, 256, 128, SPLIT, PAIRS, W>(t, st, s);
+    if (mid >= 256) return launch_product<KIND, 128, 128, SPLIT, PAIRS, W>(t, st, s);
+    return launch_product<KIND, 64, 64, SPLIT, PAIRS, W>(t, st, s);
 }
 
 } // namespace
@@ -477,6 +642,7 @@ bool launch_muon(const MuonEntry *entries, int n, DType gt, DType wt, const Muon
     t.ws = static_cast<uint8_t *>(ws);
     t.n = n;
     for (int i = 0; i < n; ++i) t.e[i] = entries[i];
+    const bool pairs = wt != DType::BF16; // three products everywhere
     const auto with_grad = [&](auto &&f) {
         switch (gt) {
             case DType::F32: return f(std::integral_constant<DType, DType::F32>{});
@@ -493,15 +659,28 @@ bool launch_muon(const MuonEntry *entries, int n, DType gt, DType wt, const Muon
             return false;
         blocks = layout(t, [](const MuonEntry &e) { return static_cast<int64_t>(e.mp / 64) * (e.np / 64); });
         if (blocks > INT32_MAX) return false;
-        return launch_ok([&] { k_muon_start<G><<<dim3(static_cast<unsigned>(blocks)), 256, 0, s>>>(t, p); });
+        return launch_ok([&] {
+            if (pairs)
+                k_muon_start<G, true><<<dim3(static_cast<unsigned>(blocks)), 256, 0, s>>>(t, p);
+            else
+                k_muon_start<G, false><<<dim3(static_cast<unsigned>(blocks)), 256, 0, s>>>(t, p);
+        });
     });
     if (!started) return false;
-    const bool split = wt != DType::BF16;
     for (int k = 0; k < p.steps; ++k) {
-        const MuonStage st{k & 1, split ? 1 : 0, k == p.steps - 1 ? 1 : 0, wt, p.a, p.b, p.c, p.decay};
-        if (!launch_stage<kGram>(t, st, split, s) || !launch_stage<kPoly>(t, st, true, s) ||
-            !launch_stage<kApply>(t, st, split, s))
-            return false;
+        const MuonStage st{k & 1, p.a, p.b, p.c, p.decay};
+        bool ok = pairs ? launch_stage<kGram, true, true>(t, st, s) && launch_stage<kPoly, true, true>(t, st, s)
+                        : launch_stage<kGram, false, false>(t, st, s) && launch_stage<kPoly, true, false>(t, st, s);
+        if (!ok) return false;
+        if (k + 1 < p.steps)
+            ok = pairs ? launch_stage<kApply, true, true>(t, st, s) : launch_stage<kApply, false, false>(t, st, s);
+        else if (wt == DType::F32)
+            ok = launch_stage<kFinal, true, true, DType::F32>(t, st, s);
+        else if (wt == DType::F16)
+            ok = launch_stage<kFinal, true, true, DType::F16>(t, st, s);
+        else
+            ok = launch_stage<kFinal, false, false, DType::BF16>(t, st, s);
+        if (!ok) return false;
     }
     return true;
 }
