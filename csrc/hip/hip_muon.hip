@@ -26,6 +26,7 @@ namespace {
 
 using half8 = _Float16 __attribute__((ext_vector_type(8)));
 using half4 = _Float16 __attribute__((ext_vector_type(4)));
+using short4v = short __attribute__((ext_vector_type(4)));
 using float16v = float __attribute__((ext_vector_type(16)));
 
 struct MuonTable {
@@ -100,6 +101,28 @@ __device__ __forceinline__ double block_sum(double v) {
     if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = v;
     __syncthreads();
     return (w[0] + w[1]) + (w[2] + w[3]);
+}
+
+// v = hi + lo, N values: one packed conversion for two, and one mixed-precision subtraction (exact) for each
+template<int N>
+__device__ __forceinline__ void split_fp16(const float (&v)[N], _Float16 __attribute__((ext_vector_type(N))) & hi,
+                                           _Float16 __attribute__((ext_vector_type(N))) & lo) {
+    using half2v = _Float16 __attribute__((ext_vector_type(2)));
+    using float2v = float __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int k = 0; k < N; k += 2) {
+        const half2v h = __builtin_convertvector((float2v{v[k], v[k + 1]}), half2v);
+        const float2v r = {__builtin_fmaf(static_cast<float>(h.x), -1.0f, v[k]),
+                           __builtin_fmaf(static_cast<float>(h.y), -1.0f, v[k + 1])};
+        const half2v l = __builtin_convertvector(r, half2v);
+        hi[k] = h.x;
+        hi[k + 1] = h.y;
+        lo[k] = l.x;
+        lo[k + 1] = l.y;
+    }
+}
+__device__ __forceinline__ float join_fp16(_Float16 hi, _Float16 lo) {
+    return __builtin_fmaf(static_cast<float>(hi), 1.0f, static_cast<float>(lo));
 }
 
 __device__ __forceinline__ float update_of(float g, float m, const MuonParams &p) {
@@ -216,10 +239,11 @@ __global__ __launch_bounds__(256) void k_muon_start(MuonTable t, MuonParams p) {
     }
     half8 hi[2], lo[2];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-        const _Float16 h = static_cast<_Float16>(v[k]);
-        hi[k / 8][k % 8] = h;
-        lo[k / 8][k % 8] = static_cast<_Float16>(v[k] - static_cast<float>(h));
+    for (int k = 0; k < 2; ++k) {
+        float part[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) part[j] = v[8 * k + j];
+        split_fp16<8>(part, hi[k], lo[k]);
     }
     _Float16 *x = q.x0 + panel_at<PAIRS>(e.mp, m0 + r, n0 + c);
     half8 *xh = reinterpret_cast<half8 *>(x), *xl = reinterpret_cast<half8 *>(x + (PAIRS ? 16 : q.xs));
@@ -247,11 +271,6 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-}
-
-__device__ __forceinline__ void split_fp16(float v, _Float16 &h, _Float16 &l) {
-    h = static_cast<_Float16>(v);
-    l = static_cast<_Float16>(v - static_cast<float>(h));
 }
 
 __device__ __forceinline__ uint32_t lds_offset(const uint8_t *p) {
@@ -444,7 +463,8 @@ __global__ __launch_bounds__(256, 2) void k_muon_product(MuonTable t, MuonStage 
     __syncthreads(); // the tiles' memory now carries results
 
     // Results leave through LDS, 32 rows of a wave at a time: a lane then has 8 neighbouring columns of a row. What it
-    // needs from memory is asked for before.
+    // needs from memory is asked for before. Of a symmetric result only the 32 x 32 blocks on and above the diagonal are
+    // used, so an entry has the same bits whatever the tile: hi lo + lo hi is not lo hi + hi lo in floating point.
     const bool flip = e.rows > e.cols;
     const int small = flip ? e.cols : e.rows, large = flip ? e.rows : e.cols;
     const int nmax = NN ? e.np : rows;
@@ -496,7 +516,7 @@ __global__ __launch_bounds__(256, 2) void k_muon_product(MuonTable t, MuonStage 
         for (int o = 0; o < O; ++o) {
             const int r = o * (64 / LR) + lane / LR, c = lane % LR * 8;
             const int m = mb + r, n = n0 + wn + c;
-            if (m >= rows || n >= nmax) continue;
+            if (m >= rows || n >= nmax || (!NN && (n | 31) < mb)) continue;
             float v[8];
             *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(slice + r * kPitch + c);
             *reinterpret_cast<float4 *>(v + 4) = *reinterpret_cast<const float4 *>(slice + r * kPitch + c + 4);
@@ -505,23 +525,17 @@ __global__ __launch_bounds__(256, 2) void k_muon_product(MuonTable t, MuonStage 
                 if constexpr (KIND == kGram) {
                     v[k] *= kMuonScaleA / (kMuonScaleX * kMuonScaleX);
                 } else {
-                    const float old = static_cast<float>(ih[o][k]) + static_cast<float>(il[o][k]);
+                    const float old = join_fp16(ih[o][k], il[o][k]);
                     if constexpr (NN)
-                        v[k] = v[k] * (1.0f / kMuonScaleP) + st.a * old;
+                        v[k] = __builtin_fmaf(st.a, old, v[k] * (1.0f / kMuonScaleP));
                     else
-                        v[k] = v[k] * (st.c * (kMuonScaleP / (kMuonScaleA * kMuonScaleA))) +
-                               (st.b * (kMuonScaleP / kMuonScaleA)) * old;
+                        v[k] = __builtin_fmaf(st.b * (kMuonScaleP / kMuonScaleA), old,
+                                              v[k] * (st.c * (kMuonScaleP / (kMuonScaleA * kMuonScaleA))));
                 }
             }
             if constexpr (KIND != kFinal) {
                 half8 oh, ol;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    _Float16 h, l;
-                    split_fp16(v[k], h, l);
-                    oh[k] = h;
-                    ol[k] = l;
-                }
+                split_fp16<8>(v, oh, ol);
                 const size_t at = panel_at<kOutPairs>(rows, m, n);
                 *reinterpret_cast<half8 *>(out + at) = oh;
                 if (lows) *reinterpret_cast<half8 *>(out + at + out_lo) = ol;
@@ -533,21 +547,18 @@ __global__ __launch_bounds__(256, 2) void k_muon_product(MuonTable t, MuonStage 
         }
         wave_sync();
         if constexpr (!NN) {
-            // the mirrored half, of tiles behind the diagonal's: 8 of the 32 rows of one column per lane
-            if (tj >= (ti + 1) * (BM / BN) && mb < rows) {
+            // the mirrored half: 8 of the 32 rows of one column per lane
+            if (n0 + wn + WN > mb + 32 && mb < rows) {
 #pragma unroll
                 for (int o = 0; o < WN; o += 16) {
                     const int c = o + (lane >> 2), r = (lane & 3) * 8;
                     const int n = n0 + wn + c;
-                    if (n >= rows) continue;
-                    half8 oh, ol;
+                    if (n >= rows || n < mb + 32) continue;
+                    float v[8];
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        _Float16 h, l;
-                        split_fp16(slice[(r + k) * kPitch + c], h, l);
-                        oh[k] = h;
-                        ol[k] = l;
-                    }
+                    for (int k = 0; k < 8; ++k) v[k] = slice[(r + k) * kPitch + c];
+                    half8 oh, ol;
+                    split_fp16<8>(v, oh, ol);
                     const size_t at = panel_at<kOutPairs>(rows, n, mb + r);
                     *reinterpret_cast<half8 *>(out + at) = oh;
                     if (lows) *reinterpret_cast<half8 *>(out + at + out_lo) = ol;
@@ -594,6 +605,289 @@ __global__ __launch_bounds__(256, 2) void k_muon_product(MuonTable t, MuonStage 
     }
 }
 
+// Everything for a matrix that fits in LDS, by one workgroup of 16 waves: X, and A / P in one place, in paired panels
+// as above and with three products throughout. The stages above would take 17 launches of a few busy CUs. Every wave
+// has one 32 x 32 tile of A or of A A; where there are only four (MP = 64), four waves each sum over a quarter of the
+// panels and then finish a quarter of the tile.
+template<int MP, int NP, DType G, DType W>
+__global__ __launch_bounds__(1024) void k_muon_small(MuonTable t, MuonParams p) {
+    using S = typename Elem<G>::S;
+    using WS = typename Elem<W>::S;
+    constexpr int MB = MP / 32;
+    constexpr int KS = 16 / (MB * MB);              // waves that share a tile of A
+    constexpr int GB = 4 / KS;                      // groups of 4 columns that a wave finishes of it
+    constexpr int AW = (MB * (NP / 32) + 15) / 16;  // tiles of X per wave
+    constexpr int E = MP * NP / 8192 > 0 ? MP * NP / 8192 : 1; // groups of 8 elements per thread
+    static_assert(MP == 64 || MP == 128);
+    __shared__ __attribute__((aligned(16))) uint8_t lx[MP * NP * 4];
+    __shared__ __attribute__((aligned(16))) uint8_t la[MP * MP * 4];
+    __shared__ float4 part[KS > 1 ? MB * MB * KS * (KS - 1) * 64 : 1];
+    __shared__ double sums[16];
+
+    const int i = entry_of(t, blockIdx.x);
+    const MuonEntry &e = t.e[i];
+    const int which = blockIdx.x - t.first[i];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int half = lane >> 5, l32 = lane & 31;
+    const size_t elems = static_cast<size_t>(e.rows) * e.cols * which;
+    const S *g = static_cast<const S *>(e.g) + elems;
+    WS *w = static_cast<WS *>(e.w) + elems;
+    float *mom = e.mom ? e.mom + elems : nullptr;
+    const bool flip = e.rows > e.cols;
+    const int np = e.np;
+
+    const int ms = flip ? e.cols : e.rows, ns = flip ? e.rows : e.cols;
+    const auto place = [&](int m, int n) { return flip ? n * e.cols + m : m * e.cols + n; };
+
+    // Momentum, and the norm; the update stays in registers, 8 neighbouring columns of a row of X per group. The lanes
+    // of a wave lie along the caller's rows: 8 x 8 groups, or 64 rows where X is the transpose.
+    float u[E][8];
+    int gm[E], gn[E];
+    bool whole[E];
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+        const int unit = threadIdx.x + 1024 * k, in = unit & 63, blk = unit >> 6;
+        gm[k] = flip ? blk % (MP / 64) * 64 + in : blk % (MP / 8) * 8 + (in >> 3);
+        gn[k] = flip ? blk / (MP / 64) * 8 : (blk / (MP / 8) * 8 + (in & 7)) * 8;
+        whole[k] = !flip && gm[k] < ms && gn[k] + 8 <= ns; // 8 neighbours in the caller's memory too
+        if (whole[k]) {
+            const Run<S, 8> v = *reinterpret_cast<const Run<S, 8> *>(g + place(gm[k], gn[k]));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) u[k][j] = static_cast<float>(v.v[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                u[k][j] = gm[k] < ms && gn[k] + j < ns ? static_cast<float>(g[place(gm[k], gn[k] + j)]) : 0.0f;
+        }
+    }
+    if (mom) {
+        Run<float, 8> old[E];
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+            if (whole[k]) {
+                old[k] = *reinterpret_cast<const Run<float, 8> *>(mom + place(gm[k], gn[k]));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    old[k].v[j] = gm[k] < ms && gn[k] + j < ns ? mom[place(gm[k], gn[k] + j)] : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float now = old[k].v[j] + (1.0f - p.momentum) * (u[k][j] - old[k].v[j]);
+                old[k].v[j] = now;
+                u[k][j] = update_of(u[k][j], now, p);
+            }
+            if (whole[k]) {
+                *reinterpret_cast<Run<float, 8> *>(mom + place(gm[k], gn[k])) = old[k];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (gm[k] < ms && gn[k] + j < ns) mom[place(gm[k], gn[k] + j)] = old[k].v[j];
+            }
+        }
+    }
+    double sum = 0.0;
+#pragma unroll
+    for (int k = 0; k < E; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += static_cast<double>(u[k][j]) * u[k][j];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    if (lane == 0) sums[wave] = sum;
+    __syncthreads();
+    sum = 0.0;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) sum += sums[k];
+    const double norm = sqrt(sum);
+    const double scale = static_cast<double>(kMuonScaleX) / (norm > p.eps || norm != norm ? norm : p.eps);
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+        if (gm[k] >= MP || gn[k] >= np) continue; // more groups than elements
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(u[k][j] * scale);
+        half8 h, l;
+        split_fp16<8>(v, h, l);
+        uint8_t *row = lx + ((gn[k] >> 4) * MP + gm[k]) * 64;
+        const int at = ((gn[k] >> 3) & 1) ^ swizzle(gm[k]);
+        *reinterpret_cast<half8 *>(row + (at << 4)) = h;
+        *reinterpret_cast<half8 *>(row + ((at ^ 2) << 4)) = l;
+    }
+
+    // What a lane adds to a tile's place: fragments of 32 rows along the sum, fragments through the transposing read,
+    // and its 4 columns of a row of a result ([lo][second 8 columns of a panel]).
+    const int sw = swizzle(l32);
+    int fo[2], to[2][2], ro[2][2];
+#pragma unroll
+    for (int lo = 0; lo < 2; ++lo) {
+        fo[lo] = l32 * 64 + (((2 * lo + half) ^ sw) << 4);
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+            const int l16 = lane & 15, r = 8 * half + 4 * z + (l16 >> 2);
+            to[z][lo] = (((lane >> 4) & 1) * MP + r) * 64 + (((2 * lo + ((l16 & 3) >> 1)) ^ swizzle(r)) << 4) + (l16 & 1) * 8;
+            ro[lo][z] = l32 * 64 + (((2 * lo + z) ^ sw) << 4) + 8 * half;
+        }
+    }
+    const auto frag = [&](const uint8_t *base, int r0, int panel, int lo) {
+        return *reinterpret_cast<const half8 *>(base + (panel * MP + r0) * 64 + fo[lo]);
+    };
+    const auto frag_t = [&](const uint8_t *base, int k0, int n0, int lo) {
+        half4 h[2];
+#pragma unroll
+        for (int z = 0; z < 2; ++z)
+            h[z] = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                 (__attribute__((address_space(3))) short4v *)(
+                                                     base + (n0 / 16 * MP + k0) * 64 + to[z][lo])));
+        return __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    const auto mul3 = [](float16v c, const half8 (&n)[2], const half8 (&m)[2]) {
+        c = __builtin_amdgcn_mfma_f32_32x32x16_f16(n[0], m[0], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_f16(n[0], m[1], c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(n[1], m[0], c, 0, 0, 0);
+    };
+    // group b of 4 columns: a result's byte without the lane's part
+    const auto group_at = [&](int mt, int nt, int b) { return ((nt / 16 + (b >> 1)) * MP + mt) * 64; };
+    const auto put4 = [&](uint8_t *base, int at, int odd, const float (&v)[4]) {
+        half4 oh, ol;
+        split_fp16<4>(v, oh, ol);
+        *reinterpret_cast<half4 *>(base + at + ro[0][odd]) = oh;
+        *reinterpret_cast<half4 *>(base + at + ro[1][odd]) = ol;
+    };
+    const auto get4 = [&](const uint8_t *base, int at, int odd, float (&v)[4]) {
+        const half4 h = *reinterpret_cast<const half4 *>(base + at + ro[0][odd]);
+        const half4 l = *reinterpret_cast<const half4 *>(base + at + ro[1][odd]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = join_fp16(h[r], l[r]);
+    };
+    // this wave's tile of `base` times its own transpose, complete in the groups GB * q ..
+    const int gt = wave % (MB * MB), gr = gt % MB * 32, gc = gt / MB * 32, gq = wave / (MB * MB);
+    const auto square = [&](const uint8_t *base, int panels, float (&out)[GB][4]) {
+        float16v acc = {};
+        for (int s = gq; s < panels; s += KS) {
+            const half8 m[2] = {frag(base, gr, s, 0), frag(base, gr, s, 1)};
+            const half8 n[2] = {frag(base, gc, s, 0), frag(base, gc, s, 1)};
+            acc = mul3(acc, n, m);
+        }
+        if constexpr (KS == 1) {
+            __syncthreads();
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) out[b][r] = acc[4 * b + r];
+        } else {
+            static_assert(KS == 4 && GB == 1);
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                if (b == gq) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) out[0][r] = acc[4 * b + r];
+                } else { // to the wave that finishes group b
+                    part[((gt * 4 + b) * 3 + (gq - b + 3) % 4) * 64 + lane] =
+                        make_float4(acc[4 * b], acc[4 * b + 1], acc[4 * b + 2], acc[4 * b + 3]);
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+                const float4 o = part[((gt * 4 + gq) * 3 + k) * 64 + lane];
+                out[0][0] += o.x;
+                out[0][1] += o.y;
+                out[0][2] += o.z;
+                out[0][3] += o.w;
+            }
+        }
+    };
+    const int tiles = MB * (np / 32);
+
+    for (int step = 0; step < p.steps; ++step) {
+        __syncthreads(); // X is written
+        float sq[GB][4];
+        square(lx, np / 16, sq);
+#pragma unroll
+        for (int k = 0; k < GB; ++k) {
+            const int b = GB * gq + k;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sq[k][r] *= kMuonScaleA / (kMuonScaleX * kMuonScaleX);
+            put4(la, group_at(gr, gc, b), b & 1, sq[k]);
+        }
+        __syncthreads(); // A is written
+        square(la, MP / 16, sq); // ends behind a barrier: A's products are read
+#pragma unroll
+        for (int k = 0; k < GB; ++k) {
+            const int b = GB * gq + k;
+            float v[4];
+            get4(la, group_at(gr, gc, b), b & 1, v); // A until here, P from now on: the same lane's
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                v[r] = __builtin_fmaf(p.b * (kMuonScaleP / kMuonScaleA), v[r],
+                                      sq[k][r] * (p.c * (kMuonScaleP / (kMuonScaleA * kMuonScaleA))));
+            put4(la, group_at(gr, gc, b), b & 1, v);
+        }
+        __syncthreads(); // P is written
+        const bool last = step == p.steps - 1;
+        float16v xa[AW];
+        Run<WS, 4> old[AW][4];
+#pragma unroll
+        for (int k = 0; k < AW; ++k) {
+            const int tile = wave + 16 * k, mt = tile % MB * 32, nt = tile / MB * 32;
+            if (tile >= tiles) break;
+            if (last && mom) {
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const int m = mt + l32, n = nt + 4 * half + 8 * b;
+                    if (!flip && m < ms && n + 4 <= ns) {
+                        old[k][b] = *reinterpret_cast<const Run<WS, 4> *>(w + place(m, n));
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) old[k][b].v[r] = m < ms && n + r < ns ? w[place(m, n + r)] : WS{};
+                    }
+                }
+            }
+            xa[k] = float16v{};
+#pragma unroll 2
+            for (int s = 0; s < MP / 16; ++s) {
+                const half8 m[2] = {frag(la, mt, s, 0), frag(la, mt, s, 1)};
+                const half8 n[2] = {frag_t(lx, 16 * s, nt, 0), frag_t(lx, 16 * s, nt, 1)};
+                xa[k] = mul3(xa[k], n, m);
+            }
+        }
+        __syncthreads(); // X is read
+#pragma unroll
+        for (int k = 0; k < AW; ++k) {
+            const int tile = wave + 16 * k, mt = tile % MB * 32, nt = tile / MB * 32;
+            if (tile >= tiles) break;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                float v[4];
+                get4(lx, group_at(mt, nt, b), b & 1, v);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = __builtin_fmaf(p.a, v[r], xa[k][4 * b + r] * (1.0f / kMuonScaleP));
+                if (!last) {
+                    put4(lx, group_at(mt, nt, b), b & 1, v);
+                    continue;
+                }
+                const int m = mt + l32, n = nt + 4 * half + 8 * b;
+                Run<WS, 4> now;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float o = v[r] * (1.0f / kMuonScaleX);
+                    now.v[r] = static_cast<WS>(mom ? static_cast<float>(old[k][b].v[r]) * p.decay - e.alpha * o : o);
+                }
+                if (!flip && m < ms && n + 4 <= ns) {
+                    *reinterpret_cast<Run<WS, 4> *>(w + place(m, n)) = now;
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (m < ms && n + r < ns) w[place(m, n + r)] = now.v[r];
+                }
+            }
+        }
+    }
+}
+
 namespace {
 
 // fills in the first workgroup of every entry; returns their number
@@ -637,11 +931,30 @@ bool launch_stage(MuonTable &t, const MuonStage &st, hipStream_t s) {
 
 } // namespace
 
+template<int MP, int NP, DType G>
+static bool launch_small(MuonTable &t, DType wt, const MuonParams &p, hipStream_t s) {
+    const int64_t n = layout(t, [](const MuonEntry &) { return 1; });
+    if (n > INT32_MAX) return false;
+    const dim3 grid(static_cast<unsigned>(n));
+    return launch_ok([&] {
+        if (wt == DType::F32)
+            k_muon_small<MP, NP, G, DType::F32><<<grid, 1024, 0, s>>>(t, p);
+        else if (wt == DType::BF16)
+            k_muon_small<MP, NP, G, DType::BF16><<<grid, 1024, 0, s>>>(t, p);
+        else
+            k_muon_small<MP, NP, G, DType::F16><<<grid, 1024, 0, s>>>(t, p);
+    });
+}
+
 bool launch_muon(const MuonEntry *entries, int n, DType gt, DType wt, const MuonParams &p, void *ws, hipStream_t s) {
-    MuonTable t{};
+    MuonTable t{}, narrow{}, square{}; // of the stages, and of one workgroup a matrix
     t.ws = static_cast<uint8_t *>(ws);
-    t.n = n;
-    for (int i = 0; i < n; ++i) t.e[i] = entries[i];
+    int np = 0;
+    for (int i = 0; i < n; ++i) {
+        MuonTable &to = !kernels::muon_fits_lds(entries[i].mp, entries[i].np) ? t : entries[i].mp == 64 ? narrow : square;
+        to.e[to.n++] = entries[i];
+        if (&to == &narrow) np = np > entries[i].np ? np : entries[i].np;
+    }
     const bool pairs = wt != DType::BF16; // three products everywhere
     const auto with_grad = [&](auto &&f) {
         switch (gt) {
@@ -653,6 +966,10 @@ bool launch_muon(const MuonEntry *entries, int n, DType gt, DType wt, const Muon
     };
     const bool started = with_grad([&](auto g) {
         constexpr DType G = decltype(g)::value;
+        if (square.n && !launch_small<128, 128, G>(square, wt, p, s)) return false;
+        if (narrow.n && !(np > 64 ? launch_small<64, 256, G>(narrow, wt, p, s) : launch_small<64, 64, G>(narrow, wt, p, s)))
+            return false;
+        if (t.n == 0) return true;
         int64_t blocks = layout(t, [](const MuonEntry &e) { return e.partials; });
         if (blocks > INT32_MAX) return false;
         if (!launch_ok([&] { k_muon_momentum<G><<<dim3(static_cast<unsigned>(blocks)), 256, 0, s>>>(t, p); }))
@@ -667,6 +984,7 @@ bool launch_muon(const MuonEntry *entries, int n, DType gt, DType wt, const Muon
         });
     });
     if (!started) return false;
+    if (t.n == 0) return true;
     for (int k = 0; k < p.steps; ++k) {
         const MuonStage st{k & 1, p.a, p.b, p.c, p.decay};
         bool ok = pairs ? launch_stage<kGram, true, true>(t, st, s) && launch_stage<kPoly, true, true>(t, st, s)

@@ -55,6 +55,9 @@ inline size_t muon_matrix_bytes(int mp, int np) {
     return 2 * (4 * static_cast<size_t>(mp) * np + 4 * static_cast<size_t>(mp) * mp) + kMuonMaxPartials * sizeof(double);
 }
 
+// matrices whose X, A and P one workgroup holds in LDS (160 KB): they need no workspace
+inline bool muon_fits_lds(int mp, int np) { return (mp == 64 && np <= 256) || (mp == 128 && np == 128); }
+
 inline int muon_pad(int64_t v) { return static_cast<int>((v + kMuonPad - 1) / kMuonPad * kMuonPad); }
 
 // Splits the entries into groups that run one after the other in the same workspace; returns the workspace's size.
@@ -73,12 +76,13 @@ inline size_t muon_plan(const std::vector<MuonEntry> &entries, size_t esize_g, s
         if (e.count == 0 || e.rows == 0 || e.cols == 0) continue;
         e.mp = muon_pad(std::min(e.rows, e.cols));
         e.np = muon_pad(std::max(e.rows, e.cols));
-        const size_t elems = static_cast<size_t>(e.rows) * e.cols, bytes = muon_matrix_bytes(e.mp, e.np);
+        const size_t elems = static_cast<size_t>(e.rows) * e.cols, bytes = muon_fits_lds(e.mp, e.np) ? 0 : muon_matrix_bytes(e.mp, e.np);
         e.partials = static_cast<int>(
             std::min<size_t>(kMuonMaxPartials, (elems + kMuonPrepBlock - 1) / kMuonPrepBlock));
         int left = e.count;
         while (left > 0) {
-            const size_t room = used < kMuonWorkspaceBudget ? (kMuonWorkspaceBudget - used) / bytes : 0;
+            size_t room = left;
+            if (bytes > 0) room = used < kMuonWorkspaceBudget ? (kMuonWorkspaceBudget - used) / bytes : 0;
             if ((room == 0 && used > 0) || static_cast<int>(group.size()) == kMuonMaxMats) {
                 flush();
                 continue;

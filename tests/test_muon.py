@@ -92,7 +92,8 @@ def check(x, got, **kw):
 
 
 SHAPES = [(1, 1), (1, 7), (7, 1), (3, 5), (64, 64), (65, 63), (100, 300), (517, 130), (2, 3, 40, 96), (5, 256, 192),
-          (1, 3001), (700, 64)]
+          (1, 3001), (700, 64),
+          (3, 256, 60), (2, 30, 250), (2, 120, 128), (64, 257)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -208,22 +209,25 @@ def test_workspace_is_bounded():
     """Large stacks run in groups: the plan's workspace stays below its budget, or is that of one matrix."""
     import ctypes
     need = lambda *s: C.pcclxMuonWorkspace(len(s) // 3, (ctypes.c_int64 * len(s))(*s))  # noqa: E731
-    one = need(1, 64, 64)
-    assert one == 2 * 8 * 64 * 64 + 4096
-    assert need(3, 64, 64) == 3 * one and need(2, 64, 64, 1, 64, 64) == 3 * one
-    assert need(1, 1, 1) == one and need(1, 65, 64) == 2 * (4 * 64 * 128 + 4 * 64 * 64) + 4096
-    assert 4 * 2 ** 30 - one < need(10 ** 6, 64, 64) <= 4 * 2 ** 30
+    one = need(1, 64, 512)
+    assert one == 2 * (4 * 64 * 512 + 4 * 64 * 64) + 4096
+    assert need(3, 512, 64) == 3 * one and need(2, 64, 512, 1, 512, 64) == 3 * one
+    assert need(1, 1, 500) == one and need(1, 65, 130) == 2 * (4 * 128 * 192 + 4 * 128 * 128) + 4096
+    assert 4 * 2 ** 30 - one < need(10 ** 6, 64, 512) <= 4 * 2 ** 30
     assert need(1, 30000, 60000) > 4 * 2 ** 30
+    for small in ((64, 64), (1, 1), (64, 256), (256, 3), (128, 128)):  # one workgroup each, in LDS
+        assert need(10 ** 6, *small) == 0
     assert need() == 0 and need(0, 5, 5) == 0
     assert need(1, -1, 5) == -1 and need(1, 2 ** 31, 5) == -1
 
 
 @pytest.mark.gpu
 def test_more_matrices_than_a_group(hip):
-    """61000 small matrices exceed the workspace's budget, 101 shapes exceed the entries of a launch."""
-    x = gradient((50, 16, 12), 8, hip).repeat(1240, 1, 1)
-    got = orthogonalize(x)
-    assert torch.equal(got, orthogonalize(x[:50]).repeat(1240, 1, 1))
+    """13100 matrices exceed the workspace's budget, 101 shapes exceed the entries of a launch."""
+    x = gradient((50, 100, 130), 8, hip)
+    assert torch.equal(orthogonalize(x.repeat(262, 1, 1)), orthogonalize(x).repeat(262, 1, 1))
+    x = x[:, :16, :12].contiguous()
+    assert torch.equal(orthogonalize(x.repeat(1240, 1, 1)), orthogonalize(x).repeat(1240, 1, 1))
     params = [torch.zeros(5 + i % 7, 3 + i, device=hip) for i in range(101)]
     grads = [gradient(p.shape, i, hip) for i, p in enumerate(params)]
     moms = [torch.zeros_like(p) for p in params]
@@ -326,22 +330,23 @@ def test_shared_gradient_and_strided_gradient(device):
 
 
 @pytest.mark.gpu
-def test_same_bits_alone_and_together(hip):
-    """A matrix's step does not depend on the others of the call, nor on the run."""
-    shapes = [(128, 64), (64, 64), (300, 500), (17, 900)]
-    grads = [gradient(s, i, hip) for i, s in enumerate(shapes)]
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_same_bits_alone_and_together(hip, dtype):
+    """A matrix's step does not depend on the others of the call (which choose the tiles), nor on the run."""
+    shapes = [(128, 64), (64, 64), (300, 500), (17, 900), (100, 128), (1000, 1500), (1100, 4000), (500, 500)]
+    grads = [gradient(s, i, hip, dtype) for i, s in enumerate(shapes)]
 
     def run(pick):
-        p = [torch.ones(shapes[i], device=hip) for i in pick]
+        p = [torch.ones(shapes[i], device=hip, dtype=dtype) for i in pick]
         b = [torch.ones(shapes[i], device=hip) for i in pick]
         muon_step(p, [grads[i] for i in pick], b, lr=0.1)
         return p + b
 
-    whole, again = run(range(4)), run(range(4))
+    whole, again = run(range(8)), run(range(8))
     assert all(torch.equal(x, y) for x, y in zip(whole, again))
-    for i in range(4):
+    for i in range(8):
         p, b = run([i])
-        assert torch.equal(p, whole[i]) and torch.equal(b, whole[4 + i])
+        assert torch.equal(p, whole[i]) and torch.equal(b, whole[8 + i])
 
 
 @pytest.mark.gpu
