@@ -279,7 +279,7 @@ PCCLX_EXPORT int pcclxTokenLogprobs(const void *logits, int64_t row_stride, int6
 // Gradient of pcclxTokenLogprobs with respect to the logits; g_* may be null (no gradient from that result).
 PCCLX_EXPORT int pcclxTokenLogprobsGrad(const void *logits, int64_t row_stride, int64_t rows, int64_t vocab, int dtype,
                                         const int64_t *targets, int64_t ignore_index, int top_k,
-                                        const float *entropy, const float *stats, const int64_t *top_index,
+                                        const float *stats, const int64_t *top_index,
                                         const float *g_logprob, const float *g_entropy, const float *g_top,
                                         void *d_logits, void *stream) {
     DeviceBackend *be = device_backend();
@@ -288,7 +288,7 @@ PCCLX_EXPORT int pcclxTokenLogprobsGrad(const void *logits, int64_t row_stride, 
         top_k > kernels::kMaxTopLogprobs || top_k > vocab)
         return -2;
     kernels::LogprobGradArgs g;
-    g.fwd = {logits, row_stride, rows, vocab, targets, ignore_index, top_k, nullptr, const_cast<float *>(entropy),
+    g.fwd = {logits, row_stride, rows, vocab, targets, ignore_index, top_k, nullptr, nullptr,
              const_cast<float *>(stats), nullptr, const_cast<int64_t *>(top_index)};
     g.g_logprob = g_logprob;
     g.g_entropy = g_entropy;

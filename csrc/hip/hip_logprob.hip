@@ -7,9 +7,9 @@
 // equal calls give equal bits.
 //
 // Top alternatives need no second pass over the row: each thread also knows its best value and the block of the row
-// where it first stood. Ordered by (value, earlier block), the k-th best of these pairs bounds the k best elements
-// from below -- each of the k better threads has an element that beats everything in a thread behind it -- so only k
-// threads look at their own elements again.
+// where it first stood, and 64 groups of threads the best of these. Ordered by (value, earlier block), the k-th best of
+// the 64 pairs bounds the k best elements from below -- each of the k better groups has an element that beats everything
+// in a group behind it -- so only threads of k groups have their elements looked at again.
 #include "dispatch.hpp"
 #include "launchers.hpp"
 
@@ -73,31 +73,26 @@ __device__ __forceinline__ uint64_t pair_key(uint32_t key, uint32_t pos) {
     return (static_cast<uint64_t>(key) << 32) | (0xffffffffu - pos);
 }
 
-// k-th largest of the R * 64 keys of one wave, 0 if fewer than k are non-zero: bit by bit over the values, then over
-// the positions of the threads that share the k-th value
-template<int R>
-__device__ uint64_t kth_largest(const uint64_t (&key)[R], int k) {
-    auto count = [&](auto &&pred) {
-        int n = 0;
-#pragma unroll
-        for (int r = 0; r < R; ++r) n += __popcll(__ballot(pred(key[r])));
-        return n;
-    };
+__device__ __forceinline__ float value_of(uint32_t key) {
+    return __builtin_bit_cast(float, (key & 0x80000000u) ? key ^ 0x80000000u : ~key);
+}
+
+// k-th largest of a wave's 64 keys, 0 if fewer than k are non-zero: bit by bit over the values, then over the positions
+// of those that share the k-th value
+__device__ uint64_t kth_largest(uint64_t key, int k) {
+    const uint32_t kh = static_cast<uint32_t>(key >> 32), kl = static_cast<uint32_t>(key);
     uint32_t hi = 0;
     for (int bit = 31; bit >= 0; --bit) {
         const uint32_t c = hi | (1u << bit);
-        if (count([&](uint64_t x) { return static_cast<uint32_t>(x >> 32) >= c; }) >= k) hi = c;
+        if (__popcll(__ballot(kh >= c)) >= k) hi = c;
     }
     if (hi == 0) return 0;
-    const int need = k - count([&](uint64_t x) { return static_cast<uint32_t>(x >> 32) > hi; });
-    if (count([&](uint64_t x) { return static_cast<uint32_t>(x >> 32) == hi; }) == need)
-        return static_cast<uint64_t>(hi) << 32;
+    const int need = k - __popcll(__ballot(kh > hi));
+    if (__popcll(__ballot(kh == hi)) == need) return static_cast<uint64_t>(hi) << 32;
     uint32_t lo = 0;
     for (int bit = 31; bit >= 0; --bit) {
         const uint32_t c = lo | (1u << bit);
-        if (count([&](uint64_t x) { return static_cast<uint32_t>(x >> 32) == hi && static_cast<uint32_t>(x) >= c; }) >=
-            need)
-            lo = c;
+        if (__popcll(__ballot(kh == hi && kl >= c)) >= need) lo = c;
     }
     return (static_cast<uint64_t>(hi) << 32) | lo;
 }
@@ -128,17 +123,15 @@ __global__ __launch_bounds__(T) void k_token_logprob(LogprobArgs a) {
 
     RowSums r{kNegInf, 0.0f, 0.0f};
     uint32_t best = tid; // block of the row where this thread's maximum first stood
-    for (int64_t b0 = tid; b0 < blocks; b0 += static_cast<int64_t>(T) * kUnroll) {
-        float v[kUnroll][W];
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) load_block<E>(x, b0 + u * T, full, a.vocab, v[u]);
+    const auto add = [&](auto &v, uint32_t b0) { // blocks b0, b0 + T, .. of this thread
+        constexpr int N = sizeof(v) / sizeof(v[0]);
         float nm = r.m;
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
+        for (int u = 0; u < N; ++u) {
             float bm = v[u][0];
 #pragma unroll
             for (int i = 1; i < W; ++i) bm = __builtin_fmaxf(bm, v[u][i]);
-            if constexpr (TOP) best = bm > nm ? static_cast<uint32_t>(b0 + u * T) : best;
+            if constexpr (TOP) best = bm > nm ? b0 + u * T : best;
             nm = __builtin_fmaxf(nm, bm);
         }
         const float mu = nm == kNegInf ? 0.0f : nm;
@@ -146,7 +139,7 @@ __global__ __launch_bounds__(T) void k_token_logprob(LogprobArgs a) {
         const float sc = __builtin_amdgcn_exp2f(dm * kLog2e);
         float s = r.s * sc, t = sc * (r.t + bounded(dm) * r.s);
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
+        for (int u = 0; u < N; ++u)
 #pragma unroll
             for (int i = 0; i < W; ++i) {
                 const float d = v[u][i] - mu;
@@ -155,6 +148,23 @@ __global__ __launch_bounds__(T) void k_token_logprob(LogprobArgs a) {
                 t = __builtin_fmaf(e, bounded(d), t);
             }
         r = {nm, s, t};
+    };
+    int64_t b0 = 0;
+    for (; b0 + kUnroll * T <= full; b0 += kUnroll * T) { // every thread has all its blocks: loads first, no branch
+        Block<S> raw[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) raw[u] = *reinterpret_cast<const Block<S> *>(x + (b0 + u * T + tid) * W);
+        float v[kUnroll][W];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[u][i] = E::ld(raw[u].v[i]);
+        add(v, static_cast<uint32_t>(b0 + tid));
+    }
+    for (int64_t b = b0 + tid; b < blocks; b += T) {
+        float v[1][W];
+        load_block<E>(x, b, full, a.vocab, v[0]);
+        add(v, static_cast<uint32_t>(b));
     }
     const RowSums mine = r;
 #pragma unroll
@@ -172,9 +182,11 @@ __global__ __launch_bounds__(T) void k_token_logprob(LogprobArgs a) {
     const float L = empty ? 0.0f : logf(r.s);
     const auto logprob_of = [&](float v) { return empty ? kNegInf : (v - r.m) - L; };
     if (tid == 0) {
-        a.stats[2 * row] = r.m;
-        a.stats[2 * row + 1] = L;
-        a.entropy[row] = empty ? 0.0f : L - r.t / r.s;
+        const float H = empty ? 0.0f : L - r.t / r.s;
+        a.stats[3 * row] = r.m;
+        a.stats[3 * row + 1] = L;
+        a.stats[3 * row + 2] = H;
+        a.entropy[row] = H;
         const int64_t t = a.targets[row];
         float lp = 0.0f;
         if (t != a.ignore_index)
@@ -182,39 +194,47 @@ __global__ __launch_bounds__(T) void k_token_logprob(LogprobArgs a) {
         a.logprob[row] = lp;
     }
     if constexpr (TOP) {
-        __shared__ uint64_t keys[T];
+        __shared__ uint64_t keys[64];
         __shared__ uint64_t cand[kCandidates];
         __shared__ uint64_t bound;
-        __shared__ int count;
+        __shared__ int count, looking;
+        __shared__ uint16_t lookers[T];
         const int k = a.top_k;
-        const uint64_t key = tid < blocks ? pair_key(order_key(mine.m), best) : 0;
-        keys[tid] = key;
+        const uint64_t own = tid < blocks ? pair_key(order_key(mine.m), best) : 0;
+        uint64_t key = own;
+#pragma unroll
+        for (int o = 1; o < kWaves; o <<= 1) { // of a group of T / 64 neighbouring threads
+            const uint64_t q = __shfl_xor(static_cast<unsigned long long>(key), o);
+            key = q > key ? q : key;
+        }
+        if (tid % kWaves == 0) keys[tid / kWaves] = key;
         __syncthreads();
         if (tid < 64) {
-            uint64_t w[kWaves];
-#pragma unroll
-            for (int i = 0; i < kWaves; ++i) w[i] = keys[i * 64 + tid];
-            const uint64_t b = kth_largest<kWaves>(w, k);
+            const uint64_t b = kth_largest(keys[tid], k);
             if (tid == 0) {
                 bound = b;
                 count = 0;
+                looking = 0;
             }
         }
         __syncthreads();
         const uint64_t bd = bound;
-        const bool looks = key != 0 && key >= bd;
-        if (looks) {
-            for (int64_t b = tid; b < blocks; b += T) {
-                float v[W];
-                load_block<E>(x, b, full, a.vocab, v);
+        const bool looks = own != 0 && own >= bd;
+        if (looks) lookers[atomicAdd(&looking, 1)] = tid;
+        __syncthreads();
+        // the lookers' blocks, shared out over the workgroup; the orders of arrival are lost in the ranks below
+        const int nl = looking, per = static_cast<int>((blocks + T - 1) / T);
+        for (int j = tid; j < nl * per; j += T) {
+            const int64_t b = lookers[j % nl] + static_cast<int64_t>(j / nl) * T;
+            if (b >= blocks) continue;
+            float v[W];
+            load_block<E>(x, b, full, a.vocab, v);
 #pragma unroll
-                for (int i = 0; i < W; ++i) {
-                    if (b * W + i >= a.vocab) break;
-                    const uint32_t ek = order_key(v[i]);
-                    if (pair_key(ek, static_cast<uint32_t>(b)) < bd) continue;
-                    const int at = atomicAdd(&count, 1); // the order of arrival is lost in the ranks below
-                    if (at < kCandidates) cand[at] = pair_key(ek, static_cast<uint32_t>(b * W + i));
-                }
+            for (int i = 0; i < W; ++i) {
+                const uint32_t ek = order_key(v[i]);
+                if (b * W + i >= a.vocab || pair_key(ek, static_cast<uint32_t>(b)) < bd) continue;
+                const int at = atomicAdd(&count, 1);
+                if (at < kCandidates) cand[at] = pair_key(ek, static_cast<uint32_t>(b * W + i));
             }
         }
         __syncthreads();
@@ -222,12 +242,13 @@ __global__ __launch_bounds__(T) void k_token_logprob(LogprobArgs a) {
         auto put = [&](int rank, uint64_t c) {
             const uint32_t idx = 0xffffffffu - static_cast<uint32_t>(c);
             a.top_index[row * k + rank] = idx;
-            a.top_logprob[row * k + rank] = logprob_of(E::ld(x[idx]));
+            a.top_logprob[row * k + rank] = logprob_of(value_of(static_cast<uint32_t>(c >> 32)));
         };
         if (n <= kCandidates) { // about k..3k of them, unless a thread holds many of the row's largest
             for (int i = tid; i < n; i += T) {
                 const uint64_t c = cand[i];
                 int rank = 0;
+#pragma unroll 8
                 for (int j = 0; j < n; ++j) rank += cand[j] > c;
                 if (rank < k) put(rank, c);
             }
@@ -278,13 +299,12 @@ __global__ __launch_bounds__(T) void k_token_logprob_grad(LogprobGradArgs g, int
     const S *x = static_cast<const S *>(a.logits) + row * a.row_stride;
     S *out = static_cast<S *>(g.d_logits) + row * a.vocab;
 
-    const float M = a.stats[2 * row], L = a.stats[2 * row + 1];
+    const float M = a.stats[3 * row], L = a.stats[3 * row + 1], H = a.stats[3 * row + 2];
     const bool empty = M == kNegInf && L == 0.0f;
     const int64_t target = a.targets[row];
     const bool has_target = target != a.ignore_index && g.g_logprob != nullptr;
     const float g_lp = has_target ? g.g_logprob[row] : 0.0f;
     const float gh = g.g_entropy ? g.g_entropy[row] : 0.0f;
-    const float H = a.entropy[row];
     float gs = g_lp;
     if (g.g_top)
         for (int k = 0; k < a.top_k; ++k) gs += g.g_top[row * a.top_k + k];
@@ -344,6 +364,7 @@ bool launch_token_logprobs(const LogprobArgs &a, DType t, hipStream_t st) {
     if (a.rows == 0) return true;
     return with_logit(t, [&](auto e) {
         using E = decltype(e);
+        constexpr int W = 16 / sizeof(typename E::S);
         const dim3 grid(static_cast<unsigned>(a.rows));
         auto run = [&](auto threads) {
             constexpr int T = decltype(threads)::value;
@@ -354,8 +375,16 @@ bool launch_token_logprobs(const LogprobArgs &a, DType t, hipStream_t st) {
                     k_token_logprob<E, T, false><<<grid, T, 0, st>>>(a);
             });
         };
-        if (a.rows <= 256) return run(std::integral_constant<int, 1024>{});
-        return run(std::integral_constant<int, 256>{});
+        // Threads per row, by its 16-byte blocks alone: enough that a thread has few to look at again for the
+        // alternatives, few enough that joining them costs little. 12288 rows, k = 0 / 20, in us with 64 / 128 / 256 /
+        // 512 threads: bf16 x 512 (64 blocks) 8 11 20 46 / 20 24 216 242; bf16 x 5000 (625) 25 25 35 60 / 48 39 55 102;
+        // bf16 x 16000 (2000) 84 83 78 111 / 134 115 98 146; bf16 x 50304 (6288) 234 237 225 220 / 444 364 279 239.
+        // One row: bf16 x 50304 18 11 7.1 6.9 / 44 20 12 10 (1024 threads: 8.5 / 12).
+        const int64_t blocks = (a.vocab + W - 1) / W;
+        if (blocks <= 256) return run(std::integral_constant<int, 64>{});
+        if (blocks <= 1024) return run(std::integral_constant<int, 128>{});
+        if (blocks <= 3000) return run(std::integral_constant<int, 256>{});
+        return run(std::integral_constant<int, 512>{});
     });
 }
 

@@ -29,7 +29,7 @@ struct LogprobArgs {
     int top_k = 0;
     float *logprob = nullptr; // [rows]
     float *entropy = nullptr; // [rows]
-    float *stats = nullptr;   // [rows, 2]: M, L (an empty row: -inf, 0)
+    float *stats = nullptr;   // [rows, 3]: M, L, H for the backward pass (an empty row: -inf, 0, 0)
     float *top_logprob = nullptr;   // [rows, top_k]
     int64_t *top_index = nullptr;   // [rows, top_k]
 };

@@ -168,7 +168,7 @@ def _load() -> ctypes.CDLL:
         "pcclxTokenLogprobs": ([c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p,
                                 c_void_p, c_void_p, c_void_p, c_void_p, c_void_p], c_int),
         "pcclxTokenLogprobsGrad": ([c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p,
-                                    c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p], c_int),
+                                    c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p], c_int),
         # Newton-Schulz orthogonalisation and the Muon step (pccl_amd.ops.muon)
         "pcclxMuonWorkspace": ([c_int, p(c_int64)], c_int64),
         "pcclxMuon": ([c_int, p(c_int64), p(c_void_p), c_int, p(c_void_p), c_int, p(c_void_p), p(c_float), c_double,

@@ -1,0 +1,26 @@
+"""Queueing a kernel on torch's current stream from Python with few host instructions: what the wrappers share."""
+from __future__ import annotations
+
+from contextlib import nullcontext
+
+import torch
+
+from .kernels import hip_device_count
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_HERE = nullcontext()
+
+
+def require_hip() -> None:
+    if hip_device_count() == 0:
+        raise RuntimeError("pccl-amd HIP backend (libpccl_hip.so) is not loaded but a GPU tensor was passed")
+
+
+def on_device(device: torch.device):
+    """A context in which ``device`` is the current one (the kernels are launched on the current device)."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def stream_of(device: torch.device) -> int:
+    """The current stream of ``device``; inside :func:`on_device`."""
+    return torch.cuda.current_stream(device).cuda_stream if _raw_stream is None else _raw_stream(device.index)

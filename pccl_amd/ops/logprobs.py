@@ -11,7 +11,8 @@ from typing import NamedTuple, Optional
 import torch
 
 from .._native import C
-from .kernels import WIRE_DTYPE, _check, hip_device_count
+from ._launch import on_device, require_hip, stream_of
+from .kernels import WIRE_DTYPE, _check
 
 MAX_TOP_LOGPROBS = 64
 
@@ -27,10 +28,15 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
-def _rows(logits: torch.Tensor) -> torch.Tensor:
-    """[rows, vocab] with the vocabulary contiguous: a view where the strides allow it, else a copy."""
-    x = logits.reshape(-1, logits.shape[-1])
-    return x if x.shape[1] == 1 or x.stride(1) == 1 else x.contiguous()
+def _rows(logits: torch.Tensor, targets: torch.Tensor):
+    """[rows, vocab] with the vocabulary contiguous and the targets in one run: views where the strides allow it, else
+    copies. (Tensors that are so already are not touched: the backward pass runs this on the autograd thread, where
+    every call into torch costs several microseconds.)"""
+    x = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
+    if x.stride(1) != 1 and x.shape[1] != 1:
+        x = x.contiguous()
+    t = targets if targets.dim() == 1 else targets.reshape(-1)
+    return x, t if t.is_contiguous() else t.contiguous()
 
 
 def _host_forward(x: torch.Tensor, targets: torch.Tensor, top_k: int, ignore_index: int):
@@ -43,7 +49,7 @@ def _host_forward(x: torch.Tensor, targets: torch.Tensor, top_k: int, ignore_ind
     empty = (m == -torch.inf) & (s == 0)
     log_s = torch.where(empty, 0.0, s.log())
     entropy = torch.where(empty, 0.0, log_s - (e * d.clamp(min=-200.0)).sum(dim=1) / s)
-    stats = torch.stack([m, log_s], dim=1)
+    stats = torch.stack([m, log_s, entropy], dim=1)
     logp = torch.where(empty[:, None], -torch.inf, (xf - m[:, None]) - log_s[:, None])
     known = (targets >= 0) & (targets < x.shape[1])
     lp = logp.gather(1, torch.where(known, targets, 0)[:, None])[:, 0]
@@ -56,18 +62,22 @@ def _host_forward(x: torch.Tensor, targets: torch.Tensor, top_k: int, ignore_ind
     return logprob, entropy, stats, top_lp, top_ix
 
 
-def _host_backward(x, targets, ignore_index, entropy, stats, top_ix, g_lp, g_h, g_top):
-    m, log_s = stats[:, :1], stats[:, 1:]
+def _host_backward(x, targets, ignore_index, stats, top_ix, g_lp, g_h, g_top):
+    m, log_s, entropy = stats.split(1, dim=1)
     empty = (m == -torch.inf) & (log_s == 0)
     logp = (x.float() - m) - log_s
-    zero = torch.zeros_like(entropy)
+    zero = torch.zeros_like(entropy[:, 0])
     used = targets != ignore_index
     known = (targets >= 0) & (targets < x.shape[1])
-    g_lp = zero if g_lp is None else torch.where(used, g_lp, 0.0)
-    g_h = zero if g_h is None else g_h
-    gs = torch.where(used & ~known, torch.nan, g_lp) + (0.0 if g_top is None else g_top.sum(dim=1))
-    d = -logp.exp() * (gs[:, None] + g_h[:, None] * (logp.clamp(min=-200.0) + entropy[:, None]))
-    d.scatter_add_(1, torch.where(known, targets, 0)[:, None], torch.where(known, g_lp, 0.0)[:, None])
+    gs = zero if g_lp is None else torch.where(used, torch.where(known, g_lp, torch.nan), 0.0)
+    at_target = zero if g_lp is None else torch.where(used & known, g_lp, 0.0)
+    if g_top is not None:
+        gs = gs + g_top.sum(dim=1)
+    term = gs[:, None]
+    if g_h is not None:
+        term = term + g_h[:, None] * (logp.clamp(min=-200.0) + entropy)
+    d = -logp.exp() * term
+    d.scatter_add_(1, torch.where(known, targets, 0)[:, None], at_target[:, None])
     if g_top is not None:
         d.scatter_add_(1, top_ix, g_top)
     return torch.where(empty, 0.0, d).to(x.dtype)
@@ -75,62 +85,78 @@ def _host_backward(x, targets, ignore_index, entropy, stats, top_ix, g_lp, g_h, 
 
 def _device_forward(x: torch.Tensor, targets: torch.Tensor, top_k: int, ignore_index: int):
     n, v = x.shape
-    logprob, entropy = (torch.empty(n, dtype=torch.float32, device=x.device) for _ in range(2))
-    stats = torch.empty((n, 2), dtype=torch.float32, device=x.device)
+    device = x.device
+    logprob = torch.empty(n, dtype=torch.float32, device=device)
+    entropy = torch.empty(n, dtype=torch.float32, device=device)
+    stats = torch.empty((n, 3), dtype=torch.float32, device=device)
     top_lp = top_ix = None
     if top_k:
-        top_lp = torch.empty((n, top_k), dtype=torch.float32, device=x.device)
-        top_ix = torch.empty((n, top_k), dtype=torch.int64, device=x.device)
+        top_lp = torch.empty((n, top_k), dtype=torch.float32, device=device)
+        top_ix = torch.empty((n, top_k), dtype=torch.int64, device=device)
     _check(C.pcclxTokenLogprobs(x.data_ptr(), x.stride(0), n, v, WIRE_DTYPE[x.dtype], targets.data_ptr(),
                                 ignore_index, top_k, logprob.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
-                                _ptr(top_lp), _ptr(top_ix), torch.cuda.current_stream(x.device).cuda_stream),
-           "token_logprobs")
+                                _ptr(top_lp), _ptr(top_ix), stream_of(device)), "token_logprobs")
     return logprob, entropy, stats, top_lp, top_ix
 
 
-def _device_backward(x, targets, ignore_index, entropy, stats, top_ix, g_lp, g_h, g_top):
+def _device_backward(x, targets, ignore_index, stats, top_ix, g_lp, g_h, g_top):
     n, v = x.shape
-    d = torch.empty((n, v), dtype=x.dtype, device=x.device)
-    g_lp, g_h, g_top = (None if g is None else g.contiguous() for g in (g_lp, g_h, g_top))
+    d = x.new_empty((n, v))
+    if g_lp is not None and not g_lp.is_contiguous():
+        g_lp = g_lp.contiguous()
+    if g_h is not None and not g_h.is_contiguous():
+        g_h = g_h.contiguous()
+    if g_top is not None and not g_top.is_contiguous():
+        g_top = g_top.contiguous()
     _check(C.pcclxTokenLogprobsGrad(x.data_ptr(), x.stride(0), n, v, WIRE_DTYPE[x.dtype], targets.data_ptr(),
-                                    ignore_index, 0 if top_ix is None else top_ix.shape[1], entropy.data_ptr(),
-                                    stats.data_ptr(), _ptr(top_ix), _ptr(g_lp), _ptr(g_h), _ptr(g_top), d.data_ptr(),
-                                    torch.cuda.current_stream(x.device).cuda_stream), "token_logprobs_grad")
+                                    ignore_index, 0 if top_ix is None else top_ix.shape[-1], stats.data_ptr(),
+                                    _ptr(top_ix), _ptr(g_lp), _ptr(g_h), _ptr(g_top), d.data_ptr(),
+                                    stream_of(x.device)), "token_logprobs_grad")
     return d
+
+
+def _forward(logits: torch.Tensor, targets: torch.Tensor, top_k: int, ignore_index: int):
+    shape = targets.shape
+    x, t = _rows(logits, targets)
+    if x.is_cuda:
+        with on_device(x.device):
+            logprob, entropy, stats, top_lp, top_ix = _device_forward(x, t, top_k, ignore_index)
+    else:
+        logprob, entropy, stats, top_lp, top_ix = _host_forward(x, t, top_k, ignore_index)
+    if len(shape) != 1:
+        logprob, entropy = logprob.view(shape), entropy.view(shape)
+        if top_k:
+            top_lp, top_ix = top_lp.view(shape + (top_k,)), top_ix.view(shape + (top_k,))
+    return logprob, entropy, stats, top_lp, top_ix
 
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top_k, ignore_index):
-        shape = targets.shape
-        x, t = _rows(logits), targets.reshape(-1).contiguous()
-        run = _device_forward if x.is_cuda else _host_forward
-        with torch.cuda.device(x.device) if x.is_cuda else torch.no_grad():
-            logprob, entropy, stats, top_lp, top_ix = run(x, t, top_k, ignore_index)
-        logprob, entropy = logprob.view(shape), entropy.view(shape)
+        logprob, entropy, ctx.stats, top_lp, top_ix = _forward(logits, targets, top_k, ignore_index)
         if top_k:
-            top_lp, top_ix = top_lp.view(shape + (top_k,)), top_ix.view(shape + (top_k,))
             ctx.mark_non_differentiable(top_ix)
         ctx.ignore_index = ignore_index
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(logits, t, entropy, stats, top_ix)
+        ctx.save_for_backward(logits, targets, top_ix)
         return logprob, entropy, top_lp, top_ix
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_lp, g_h, g_top, _):
-        logits, t, entropy, stats, top_ix = ctx.saved_tensors
+        logits, targets, top_ix = ctx.saved_tensors
         if g_lp is None and g_h is None and g_top is None:
             return None, None, None, None
-        x = _rows(logits)
-        flat = lambda g: None if g is None else g.reshape(-1)  # noqa: E731
-        if top_ix is not None:
-            top_ix = top_ix.reshape(len(t), -1)
-            g_top = None if g_top is None else g_top.reshape(len(t), -1)
-        run = _device_backward if x.is_cuda else _host_backward
-        with torch.cuda.device(x.device) if x.is_cuda else torch.no_grad():
-            d = run(x, t, ctx.ignore_index, entropy.reshape(-1), stats, top_ix, flat(g_lp), flat(g_h), g_top)
-        return d.view(logits.shape), None, None, None
+        x, t = _rows(logits, targets)
+        if logits.dim() != 2:
+            g_lp, g_h = (None if g is None else g.reshape(-1) for g in (g_lp, g_h))
+            top_ix, g_top = (None if v is None else v.reshape(-1, v.shape[-1]) for v in (top_ix, g_top))
+        if x.is_cuda:
+            with on_device(x.device):
+                d = _device_backward(x, t, ctx.ignore_index, ctx.stats, top_ix, g_lp, g_h, g_top)
+        else:
+            d = _host_backward(x, t, ctx.ignore_index, ctx.stats, top_ix, g_lp, g_h, g_top)
+        return d if logits.dim() == 2 else d.view(logits.shape), None, None, None
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top_k: int = 0,
@@ -167,8 +193,10 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top_k: int = 
     if targets.numel() >= 1 << 31 or logits.shape[-1] >= 1 << 31:
         raise ValueError("token_logprobs: at most 2^31 - 1 rows and tokens of vocabulary")
     if logits.device.type == "cuda":
-        if hip_device_count() == 0:
-            raise RuntimeError("pccl-amd HIP backend (libpccl_hip.so) is not loaded but a GPU tensor was passed")
+        require_hip()
     elif logits.device.type != "cpu":
         raise ValueError(f"token_logprobs: no kernel for device {logits.device}")
-    return TokenLogprobs(*_TokenLogprobs.apply(logits, targets, int(top_k), int(ignore_index)))
+    if logits.requires_grad and torch.is_grad_enabled():
+        return TokenLogprobs(*_TokenLogprobs.apply(logits, targets, int(top_k), int(ignore_index)))
+    logprob, entropy, _, top_lp, top_ix = _forward(logits, targets, int(top_k), int(ignore_index))
+    return TokenLogprobs(logprob, entropy, top_lp, top_ix)

@@ -16,7 +16,8 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from .._native import C
-from .kernels import WIRE_DTYPE, _check, hip_device_count
+from ._launch import on_device, require_hip, stream_of
+from .kernels import WIRE_DTYPE, _check
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 _TYPES = (torch.float32, torch.bfloat16, torch.float16)
@@ -53,26 +54,29 @@ def _host_orthogonalize(x: torch.Tensor, steps: int, coefficients, eps: float) -
     return y.mT if flip else y
 
 
-def _queue(entries, gtype, wtype, mom, alpha, decay, momentum, nesterov, steps, coefficients, eps, device, what):
-    """entries: (count, rows, cols, g, w) with tensors g and w; mom: tensors or None."""
-    if hip_device_count() == 0:
-        raise RuntimeError("pccl-amd HIP backend (libpccl_hip.so) is not loaded but a GPU tensor was passed")
-    n = len(entries)
-    shapes = (ctypes.c_int64 * (3 * n))(*[v for e in entries for v in e[:3]])
+def _queue(shapes, g, gtype, w, wtype, mom, alpha, decay, momentum, nesterov, steps, coefficients, eps, device, what):
+    """shapes: count, rows, cols of each entry, flat; g, w and mom (None: orthogonalise): addresses."""
+    require_hip()
+    n = len(g)
+    shapes = (ctypes.c_int64 * (3 * n))(*shapes)
+    pointers = ctypes.c_void_p * n
     need = C.pcclxMuonWorkspace(n, shapes)
     if need < 0:
         raise ValueError(f"{what}: a matrix is too large")
-    pointers = lambda ts: (ctypes.c_void_p * n)(*[t.data_ptr() for t in ts])  # noqa: E731
-    with torch.cuda.device(device):
-        work = torch.empty(need, dtype=torch.uint8, device=device)
-        rc = C.pcclxMuon(n, shapes, pointers(e[3] for e in entries), WIRE_DTYPE[gtype],
-                         pointers(e[4] for e in entries), WIRE_DTYPE[wtype], pointers(mom) if mom else None,
-                         (ctypes.c_float * n)(*alpha) if alpha else None, decay, momentum, int(nesterov), steps,
-                         (ctypes.c_float * 3)(*coefficients), eps, work.data_ptr(), need,
-                         torch.cuda.current_stream(device).cuda_stream)
+    with on_device(device):
+        work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        rc = C.pcclxMuon(n, shapes, pointers(*g), WIRE_DTYPE[gtype], pointers(*w), WIRE_DTYPE[wtype],
+                         pointers(*mom) if mom else None, (ctypes.c_float * n)(*alpha) if mom else None, decay,
+                         momentum, nesterov, steps, _floats(coefficients), eps, work.data_ptr() if need else None, need,
+                         stream_of(device))
     if rc == -3:
         raise ValueError(f"{what}: a tensor that is written shares memory with another one of the call")
     _check(rc, what)
+
+
+@lru_cache(maxsize=64)
+def _floats(coefficients: Tuple[float, ...]):
+    return (ctypes.c_float * 3)(*coefficients)
 
 
 def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence[float] = COEFFICIENTS,
@@ -84,8 +88,8 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence[flo
     result one rounding more than bf16's own. A zero matrix gives zero, one with a NaN or an infinity gives NaN.
     Non-contiguous input is copied. ``out`` (contiguous, of x's shape and type) may be ``x`` itself.
     """
-    coefficients = tuple(float(v) for v in coefficients)
-    _check_coefficients(coefficients, int(steps))
+    coefficients, steps = tuple(coefficients), int(steps)
+    _check_coefficients(coefficients, steps)
     if x.dim() < 2:
         raise ValueError(f"orthogonalize: a matrix or a stack of them, got shape {tuple(x.shape)}")
     if x.dtype not in _TYPES:
@@ -101,12 +105,14 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence[flo
     if x.numel() == 0:
         return out
     if x.device.type == "cpu":
-        return out.copy_(_host_orthogonalize(x, int(steps), coefficients, eps))
+        return out.copy_(_host_orthogonalize(x, steps, coefficients, eps))
     if x.device.type != "cuda":
         raise ValueError(f"orthogonalize: no kernel for device {x.device}")
     m, n = x.shape[-2:]
-    _queue([(x.numel() // (m * n), m, n, x.contiguous(), out)], x.dtype, out.dtype, None, None, 1.0, 0.0, False,
-           int(steps), coefficients, float(eps), x.device, "orthogonalize")
+    x = x.contiguous()
+    _queue((x.numel() // (m * n), m, n), (x.data_ptr(),), x.dtype, (out.data_ptr(),), x.dtype, None, None, 1.0, 0.0, 0,
+           steps, coefficients, eps, x.device, "orthogonalize")
+    torch.autograd.graph.increment_version(out)
     return out
 
 
@@ -136,8 +142,8 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     non-contiguous ones are copied; ``momentum_buffers``: contiguous fp32. All on one device, none of them sharing
     memory with another (a parameter listed twice is refused). Equal calls give equal bits on every peer.
     """
-    coefficients = tuple(float(v) for v in coefficients)
-    _check_coefficients(coefficients, int(steps))
+    coefficients, steps = tuple(coefficients), int(steps)
+    _check_coefficients(coefficients, steps)
     if not len(params) == len(grads) == len(momentum_buffers):
         raise ValueError(f"muon_step: {len(params)} parameters, {len(grads)} gradients and {len(momentum_buffers)} "
                          "momentum buffers")
@@ -155,10 +161,11 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
         raise TypeError(f"muon_step: fp32/bf16/fp16 parameters and gradients, got {wtype} and {gtype}")
     if device.type not in ("cpu", "cuda"):
         raise ValueError(f"muon_step: no kernel for device {device}")
-    entries, moms, alpha = [], [], []
+    work = []
     for p, g, b in zip(params, grads, momentum_buffers):
-        if p.dim() != 2 or p.shape != g.shape or p.shape != b.shape:
-            raise ValueError(f"muon_step: matrices of one shape, got parameter {tuple(p.shape)}, gradient "
+        shape = p.shape
+        if len(shape) != 2 or shape != g.shape or shape != b.shape:
+            raise ValueError(f"muon_step: matrices of one shape, got parameter {tuple(shape)}, gradient "
                              f"{tuple(g.shape)}, momentum {tuple(b.shape)}")
         if p.dtype != wtype or g.dtype != gtype:
             raise TypeError("muon_step: parameters, and gradients, must be of one type each")
@@ -168,28 +175,30 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
             raise ValueError("muon_step: every tensor must be on one device")
         if not p.is_contiguous() or not b.is_contiguous():
             raise ValueError("muon_step: parameters and momentum buffers must be contiguous")
-        if p.numel() == 0:
-            continue
-        entries.append((1, p.shape[0], p.shape[1], g.detach().contiguous(), p))
-        moms.append(b)
-        alpha.append(lr * _shape_factor(p.shape[0], p.shape[1], adjust_lr))
-    if not entries:
+        rows, cols = shape
+        if rows and cols:
+            work.append((rows, cols, p, g if g.is_contiguous() else g.detach().contiguous(), b))
+    if not work:
         return
+    factors = {}
+    for e in work:
+        if e[:2] not in factors:
+            factors[e[:2]] = lr * _shape_factor(*e[:2], adjust_lr)
+    alpha = [factors[e[:2]] for e in work]
     decay = 1.0 - lr * weight_decay
     if device.type == "cuda":
-        _queue(entries, gtype, wtype, moms, alpha, decay, momentum, nesterov, int(steps), coefficients, float(eps),
-               device, "muon_step")
-        for p, b in zip(params, momentum_buffers):
-            torch.autograd.graph.increment_version(p)
-            torch.autograd.graph.increment_version(b)
+        _queue([v for e in work for v in (1, e[0], e[1])], [e[3].data_ptr() for e in work], gtype,
+               [e[2].data_ptr() for e in work], wtype, [e[4].data_ptr() for e in work], alpha, decay, momentum,
+               int(nesterov), steps, coefficients, eps, device, "muon_step")
+        torch.autograd.graph.increment_version([t for e in work for t in (e[2], e[4])])
         return
     with torch.no_grad():
-        written = [t for e, b in zip(entries, moms) for t in (e[4], b)]
+        written = [t for e in work for t in (e[2], e[4])]
         spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in written)
         if any(x[1] > y[0] for x, y in zip(spans, spans[1:])):
             raise ValueError("muon_step: a tensor that is written shares memory with another one of the call")
-        for (_, _, _, g, p), b, al in zip(entries, moms, alpha):
+        for (_, _, p, g, b), al in zip(work, alpha):
             g = g.float()
             b.add_(g - b, alpha=1.0 - momentum)
             u = g + momentum * (b - g) if nesterov else b
-            p.copy_(p.float() * decay - al * _host_orthogonalize(u, int(steps), coefficients, eps))
+            p.copy_(p.float() * decay - al * _host_orthogonalize(u, steps, coefficients, eps))
