@@ -9,6 +9,8 @@
 // The products of the 16-bit types: where the result is bf16 (8 bits), A and P X use the hi parts alone (11 bits) and
 // only A A, the cheapest, all three; the term a X always has both parts, so small singular values, which the steps
 // amplify up to a^steps, keep their precision. Other results use three products everywhere, the error of fp32 products.
+#include <algorithm>
+
 #include "dispatch.hpp"
 #include "launchers.hpp"
 
@@ -39,6 +41,7 @@ static_assert(sizeof(MuonTable) < 4000, "kernel arguments");
 
 // entry of workgroup `b`: the lanes compare one entry each
 __device__ __forceinline__ int entry_of(const MuonTable &t, int b) {
+    if (t.n == 1) return 0;
     const int lane = threadIdx.x & 63;
     const bool before = lane < t.n && t.first[lane < t.n ? lane : 0] <= b;
     return __builtin_amdgcn_readfirstlane(__popcll(__ballot(before)) - 1);
@@ -260,11 +263,19 @@ struct MuonStage {
     float a, b, c, decay;
 };
 
-constexpr int kStages = 3; // tiles of the sum in LDS: one is multiplied, two are on their way
-
 template<int N>
 __device__ __forceinline__ void wait_loads() { // all but the N newest loads of this wave have landed, its LDS reads too
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
+// the same with N per tile and `tiles` < LEFT tiles still allowed to be on their way
+template<int N, int LEFT>
+__device__ __forceinline__ void wait_tiles(int tiles) {
+    if constexpr (LEFT > 0) {
+        if (tiles >= LEFT - 1)
+            wait_loads<N * (LEFT - 1)>();
+        else
+            wait_tiles<N, LEFT - 1>(tiles);
+    }
 }
 // orders LDS accesses between the lanes of one wave
 __device__ __forceinline__ void wave_sync() {
@@ -314,28 +325,40 @@ __device__ __forceinline__ void read_transposed(uint32_t base, const uint32_t (&
         for (int s = 0; s < 2; ++s) f[y][s] = __builtin_shufflevector(h[y][0][s], h[y][1][s], 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// 16-byte pieces of a panel's 64-byte rows trade places in LDS by the row: a fragment's reads (one piece of 8 rows, or
-// two of 4) then meet no bank twice
-__device__ __forceinline__ int swizzle(int r) { return (r & 2) | ((r >> 2) & 1); }
+// 16-byte pieces of a panel's 64-byte rows trade places in LDS: a fragment's 16-byte reads are served 16 rows at a time
+// from 64 banks, so rows 4 apart must differ; the transposing read takes 4 rows of two column blocks at a time, and
+// where these lie in two panels their pieces must differ too.
+__device__ __forceinline__ int swizzle(int r) { return (r >> 2) & 3; }
+__device__ __forceinline__ int swizzle(int r, int panel) { return swizzle(r) ^ ((panel & 1) << 1); }
+
+// Work item of this workgroup. Workgroups go to the 8 chiplets in turn; each gets runs of kRun neighbouring tiles, which
+// share operands in its L2, and the runs advance together, because the items are sorted by falling length.
+constexpr int kRun = 32;
+__device__ __forceinline__ int place_of_block() {
+    const int b = blockIdx.x, n = gridDim.x, window = 8 * kRun;
+    const int base = b / window * window, run = n - base < window ? (n - base) / 8 : kRun;
+    const int k = b - base;
+    return k < 8 * run ? base + (k & 7) * run + (k >> 3) : b;
+}
 
 // One product stage. A workgroup computes BM x BN of it. The M side's rows (of X, A or P) lie along the sum, and so do
 // the N side's of kGram and kPoly, which multiply by a transpose; kApply's and kFinal's N side is X itself, whose
 // fragments are transposed on their way out of LDS. Both sides travel straight to LDS, a panel of the sum at a time.
 // SPLIT: three products of the parts. PAIRS: X and P lie in pairs. The MFMA's first operand is the N side: a lane then
 // holds 4 neighbouring columns of one row.
-template<int KIND, int BM, int BN, bool SPLIT, bool PAIRS, DType W>
-__global__ __launch_bounds__(256, 2) void k_muon_product(MuonTable t, MuonStage st) {
+// KG groups of four waves take the panels in turn and add their sums up at the end: with few tiles this fills the CUs.
+// Of ST panels in a group's part of LDS one is multiplied, the others are on their way.
+template<int KIND, int BM, int BN, int KG, int ST, bool SPLIT, bool PAIRS, DType W>
+__global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void k_muon_product(MuonTable t, MuonStage st) {
     constexpr int WM = BM / 2, WN = BN / 2, MT = WM / 32, NT = WN / 32;
     constexpr int BK = SPLIT ? 16 : 32; // columns of a panel, the step along the sum
     constexpr bool NN = KIND == kApply || KIND == kFinal;
     constexpr int kTile = (BM + BN) * 64;
     constexpr int kSlice = 32 * (WN + 4) * 4; // 32 rows of a wave's results, padded against bank conflicts
-    constexpr int kLds = kStages * kTile > 4 * kSlice ? kStages * kTile : 4 * kSlice;
+    constexpr int kLds = KG * (ST * kTile > 4 * kSlice ? ST * kTile : 4 * kSlice);
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
 
-    const int per_xcd = gridDim.x / 8; // workgroups of one matrix next to each other on one chiplet's L2
-    const int blk = static_cast<int>(blockIdx.x) < per_xcd * 8 ? (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3)
-                                                                 : static_cast<int>(blockIdx.x);
+    const int blk = place_of_block();
     const int i = entry_of(t, blk);
     const MuonEntry &e = t.e[i];
     const int rows = e.mp;
@@ -363,31 +386,33 @@ __global__ __launch_bounds__(256, 2) void k_muon_product(MuonTable t, MuonStage 
     const _Float16 *ms = KIND == kGram ? x : KIND == kPoly ? q.a : q.p;
     const _Float16 *ns = KIND == kPoly ? q.a : x;
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) & 3, group = threadIdx.x >> 8;
     // source of each 16-byte piece this lane brings to LDS; rows and panels past the matrix repeat its last ones
     constexpr int MI = BM / 64, NI = BN / 64;
     const _Float16 *mp[MI], *np[NI];
     const int lrow = lane >> 2;
-    const int lpiece = ((lane & 3) ^ swizzle(lrow)) * 8;
+    const int lpiece = (lane & 3) ^ swizzle(lrow);
 #pragma unroll
     for (int k = 0; k < MI; ++k) {
         const int r = m0 + (wave * MI + k) * 16 + lrow;
-        mp[k] = ms + static_cast<size_t>(r < rows ? r : rows - 1) * 32 + lpiece;
+        mp[k] = ms + (static_cast<size_t>(group) * rows + (r < rows ? r : rows - 1)) * 32 + lpiece * 8;
     }
 #pragma unroll
     for (int k = 0; k < NI; ++k) {
         if constexpr (NN) { // BK rows of BN / BK panels
             const int j = wave * NI + k, panels = e.np / BK;
             const int pn = n0 / BK + j / (BK / 16);
-            np[k] = ns + (static_cast<size_t>(pn < panels ? pn : panels - 1) * rows + j % (BK / 16) * 16 + lrow) * 32 + lpiece;
+            np[k] = ns + (static_cast<size_t>(pn < panels ? pn : panels - 1) * rows + group * BK + j % (BK / 16) * 16 + lrow) * 32 +
+                    (lpiece ^ (SPLIT ? (j & 1) << 1 : 0)) * 8;
         } else {
             const int r = n0 + (wave * NI + k) * 16 + lrow;
-            np[k] = ns + static_cast<size_t>(r < rows ? r : rows - 1) * 32 + lpiece;
+            np[k] = ns + (static_cast<size_t>(group) * rows + (r < rows ? r : rows - 1)) * 32 + lpiece * 8;
         }
     }
-    const size_t mstep = static_cast<size_t>(rows) * 32, nstep = NN ? BK * 32 : mstep;
+    const size_t mstep = static_cast<size_t>(rows) * 32 * KG, nstep = NN ? BK * 32 * KG : mstep;
+    uint8_t *mine = lds + group * ST * kTile;
     const auto fetch = [&](int buf) {
-        uint8_t *to = lds + buf * kTile;
+        uint8_t *to = mine + buf * kTile;
 #pragma unroll
         for (int k = 0; k < MI; ++k) {
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)mp[k],
@@ -416,21 +441,44 @@ __global__ __launch_bounds__(256, 2) void k_muon_product(MuonTable t, MuonStage 
                 const int r = 8 * half + 4 * z + (l16 >> 2) + (SPLIT ? 0 : 16 * s);
                 const int piece = (SPLIT ? 2 * s : 2 * cb) + ((l16 & 3) >> 1);
                 const int panel = SPLIT ? wn / 16 + cb : wn / 32;
-                tr[z][s] = panel * (BK * 64) + r * 64 + ((piece ^ swizzle(r)) << 4) + (l16 & 1) * 8;
+                tr[z][s] = panel * (BK * 64) + r * 64 + ((piece ^ swizzle(r, SPLIT ? cb : 0)) << 4) + (l16 & 1) * 8;
             }
     }
+    constexpr bool kInPairs = NN ? PAIRS : true;  // layout of what the epilogue reads (X, or A)
+    const size_t in_lo = kInPairs ? 16 : q.xs;
+    const _Float16 *in = NN ? x : q.a;
+    const int nmax = NN ? e.np : rows;
+    constexpr int LR = WN / 8, O = 32 / (64 / LR); // lanes of a row, and pieces of a slice of 32 rows of the results
+    const auto mine_of = [&](int o) { return KG == 1 || o % KG == group; }; // pieces are shared out over the groups
+    const auto ask = [&](int u, half8 (&ih)[O], half8 (&il)[O]) {
+#pragma unroll
+        for (int o = 0; o < O; ++o) {
+            const int m = m0 + wm + u * 32 + o * (64 / LR) + lane / LR, n = n0 + wn + lane % LR * 8;
+            if (mine_of(o) && m < rows && n < nmax) {
+                const size_t at = panel_at<kInPairs>(rows, m, n);
+                ih[o] = *reinterpret_cast<const half8 *>(in + at);
+                il[o] = *reinterpret_cast<const half8 *>(in + at + in_lo);
+            }
+        }
+    };
+    constexpr bool kAskFirst = KIND != kGram && KG > 1; // few tiles: nothing else would hide these loads
+    half8 eh[kAskFirst ? MT : 1][O], el[kAskFirst ? MT : 1][O];
+    if constexpr (kAskFirst) {
+#pragma unroll
+        for (int u = 0; u < MT; ++u) ask(u, eh[u], el[u]);
+    }
     float16v acc[NT][MT] = {};
-    const int steps = K / BK; // K is a multiple of 64
-    fetch(0);
-    fetch(1);
-    for (int k = 0, buf = 0; k < steps; ++k) {
-        if (k + 1 < steps)
-            wait_loads<MI + NI>();
-        else
-            wait_loads<0>();
+    const int panels = K / BK, rounds = (panels + KG - 1) / KG, steps = (panels - group + KG - 1) / KG; // this group's
+#pragma unroll
+    for (int k = 0; k < ST - 1; ++k)
+        if (k < steps) fetch(k);
+    for (int k = 0, buf = 0, to = ST - 1; k < rounds; ++k) {
+        const int later = steps - 1 - k; // tiles behind this one
+        wait_tiles<MI + NI, ST - 1>(later < ST - 2 ? (later > 0 ? later : 0) : ST - 2);
         __builtin_amdgcn_s_barrier(); // tile k has landed for every wave, and all are done with tile k - 1
         asm volatile("" ::: "memory");
-        const uint8_t *ml = lds + buf * kTile, *nl = ml + BM * 64;
+        if (KG > 1 && k >= steps) break; // the last round, without a panel for this group
+        const uint8_t *ml = mine + buf * kTile, *nl = ml + BM * 64;
         half8 mf[MT][2], nf[NT][2]; // two pieces of 16 of the sum: hi and lo of one, or both of 32
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -443,8 +491,9 @@ __global__ __launch_bounds__(256, 2) void k_muon_product(MuonTable t, MuonStage 
             }
         }
         if constexpr (NN) read_transposed<NT, 32 / BK * BK * 64>(lds_offset(nl), tr, nf);
-        buf = buf == kStages - 1 ? 0 : buf + 1;
-        if (k + 2 < steps) fetch(buf == kStages - 1 ? 0 : buf + 1); // over tile k - 1
+        if (k + ST - 1 < steps) fetch(to); // over tile k - 1
+        buf = buf == ST - 1 ? 0 : buf + 1;
+        to = to == ST - 1 ? 0 : to + 1;
         const auto mul = [&](int sn, int sm) {
 #pragma unroll
             for (int y = 0; y < NT; ++y)
@@ -464,13 +513,19 @@ __global__ __launch_bounds__(256, 2) void k_muon_product(MuonTable t, MuonStage 
 
     // Results leave through LDS, 32 rows of a wave at a time: a lane then has 8 neighbouring columns of a row. What it
     // needs from memory is asked for before. Of a symmetric result only the 32 x 32 blocks on and above the diagonal are
-    // used, so an entry has the same bits whatever the tile: hi lo + lo hi is not lo hi + hi lo in floating point.
+    // used: hi lo + lo hi is not lo hi + hi lo in floating point, and the mirrored half comes from the other.
     const bool flip = e.rows > e.cols;
     const int small = flip ? e.cols : e.rows, large = flip ? e.rows : e.cols;
-    const int nmax = NN ? e.np : rows;
-    constexpr int LR = WN / 8, O = 32 / (64 / LR); // lanes of a row, and pieces of a slice
     constexpr int kPitch = WN + 4;
+    // a wave's slice of its own sums, the first group's (the whole sum's), and what orders accesses to them
+    float *own = reinterpret_cast<float *>(lds + (group * 4 + wave) * kSlice);
     float *slice = reinterpret_cast<float *>(lds + wave * kSlice);
+    const auto sync = [] {
+        if constexpr (KG == 1)
+            wave_sync();
+        else
+            __syncthreads();
+    };
     using WS = typename Elem<W>::S;
     WS *w = KIND == kFinal ? static_cast<WS *>(e.w) + static_cast<size_t>(e.rows) * e.cols * which : nullptr;
     const float alpha = e.alpha;
@@ -479,26 +534,22 @@ __global__ __launch_bounds__(256, 2) void k_muon_product(MuonTable t, MuonStage 
         v *= 1.0f / kMuonScaleX;
         return static_cast<WS>(step ? static_cast<float>(old) * st.decay - alpha * v : v);
     };
-    constexpr bool kInPairs = NN ? PAIRS : true;  // layout of what the epilogue reads (X, or A)
-    constexpr bool kOutPairs = KIND == kGram || PAIRS; // and writes (A, P or X)
-    const size_t in_lo = kInPairs ? 16 : q.xs, out_lo = kOutPairs ? 16 : q.xs;
-    const _Float16 *in = NN ? x : q.a;
+    constexpr bool kOutPairs = KIND == kGram || PAIRS; // layout of what is written (A, P or X)
+    const size_t out_lo = kOutPairs ? 16 : q.xs;
     _Float16 *out = KIND == kGram ? q.a : KIND == kPoly ? q.p : st.cur ? q.x0 : q.x1;
     const bool lows = KIND != kPoly || PAIRS; // P's lo parts are only there to be multiplied
 #pragma unroll
     for (int u = 0; u < MT; ++u) {
         const int mb = m0 + wm + u * 32;
         half8 ih[O], il[O];
-        if constexpr (KIND != kGram) {
+        if constexpr (kAskFirst) {
 #pragma unroll
             for (int o = 0; o < O; ++o) {
-                const int m = mb + o * (64 / LR) + lane / LR, n = n0 + wn + lane % LR * 8;
-                if (m < rows && n < nmax) {
-                    const size_t at = panel_at<kInPairs>(rows, m, n);
-                    ih[o] = *reinterpret_cast<const half8 *>(in + at);
-                    il[o] = *reinterpret_cast<const half8 *>(in + at + in_lo);
-                }
+                ih[o] = eh[u][o];
+                il[o] = el[u][o];
             }
+        } else if constexpr (KIND != kGram) {
+            ask(u, ih, il);
         }
 #pragma unroll
         for (int y = 0; y < NT; ++y)
@@ -509,17 +560,23 @@ __global__ __launch_bounds__(256, 2) void k_muon_product(MuonTable t, MuonStage 
                 v.y = acc[y][u][4 * k + 1];
                 v.z = acc[y][u][4 * k + 2];
                 v.w = acc[y][u][4 * k + 3];
-                *reinterpret_cast<float4 *>(slice + l32 * kPitch + y * 32 + 8 * k + 4 * half) = v;
+                *reinterpret_cast<float4 *>(own + l32 * kPitch + y * 32 + 8 * k + 4 * half) = v;
             }
-        wave_sync();
+        sync();
 #pragma unroll
         for (int o = 0; o < O; ++o) {
             const int r = o * (64 / LR) + lane / LR, c = lane % LR * 8;
             const int m = mb + r, n = n0 + wn + c;
-            if (m >= rows || n >= nmax || (!NN && (n | 31) < mb)) continue;
+            if (!mine_of(o) || m >= rows || n >= nmax || (!NN && (n | 31) < mb)) continue;
             float v[8];
             *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(slice + r * kPitch + c);
             *reinterpret_cast<float4 *>(v + 4) = *reinterpret_cast<const float4 *>(slice + r * kPitch + c + 4);
+#pragma unroll
+            for (int j = 1; j < KG; ++j) {
+                const float *other = slice + j * kSlice + r * kPitch + c; // 4 slices a group, 4 bytes an element
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] += other[k];
+            }
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 if constexpr (KIND == kGram) {
@@ -545,7 +602,7 @@ __global__ __launch_bounds__(256, 2) void k_muon_product(MuonTable t, MuonStage 
                 *reinterpret_cast<float4 *>(slice + r * kPitch + c + 4) = *reinterpret_cast<float4 *>(v + 4);
             }
         }
-        wave_sync();
+        sync();
         if constexpr (!NN) {
             // the mirrored half: 8 of the 32 rows of one column per lane
             if (n0 + wn + WN > mb + 32 && mb < rows) {
@@ -553,7 +610,7 @@ __global__ __launch_bounds__(256, 2) void k_muon_product(MuonTable t, MuonStage 
                 for (int o = 0; o < WN; o += 16) {
                     const int c = o + (lane >> 2), r = (lane & 3) * 8;
                     const int n = n0 + wn + c;
-                    if (n >= rows || n < mb + 32) continue;
+                    if (!mine_of(o / 16) || n >= rows || n < mb + 32) continue;
                     float v[8];
 #pragma unroll
                     for (int k = 0; k < 8; ++k) v[k] = slice[(r + k) * kPitch + c];
@@ -578,10 +635,11 @@ __global__ __launch_bounds__(256, 2) void k_muon_product(MuonTable t, MuonStage 
                 const int n = flip ? n0 + wn + lr + 8 * k : n0 + wn + lc;
                 at[k] = flip ? static_cast<size_t>(n) * e.cols + m : static_cast<size_t>(m) * e.cols + n;
                 whole[k] = flip ? n < large && m + 4 <= small : m < small && n + 4 <= large;
-                if (whole[k] && step) old[k] = *reinterpret_cast<const Run<WS, 4> *>(w + at[k]);
+                if (mine_of(k) && whole[k] && step) old[k] = *reinterpret_cast<const Run<WS, 4> *>(w + at[k]);
             }
 #pragma unroll
             for (int k = 0; k < P; ++k) {
+                if (!mine_of(k)) continue;
                 float v[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
@@ -601,7 +659,7 @@ __global__ __launch_bounds__(256, 2) void k_muon_product(MuonTable t, MuonStage 
                 }
             }
         }
-        wave_sync();
+        sync();
     }
 }
 
@@ -712,27 +770,29 @@ __global__ __launch_bounds__(1024) void k_muon_small(MuonTable t, MuonParams p) 
         half8 h, l;
         split_fp16<8>(v, h, l);
         uint8_t *row = lx + ((gn[k] >> 4) * MP + gm[k]) * 64;
-        const int at = ((gn[k] >> 3) & 1) ^ swizzle(gm[k]);
+        const int at = ((gn[k] >> 3) & 1) ^ swizzle(gm[k], gn[k] >> 4);
         *reinterpret_cast<half8 *>(row + (at << 4)) = h;
         *reinterpret_cast<half8 *>(row + ((at ^ 2) << 4)) = l;
     }
 
     // What a lane adds to a tile's place: fragments of 32 rows along the sum, fragments through the transposing read,
-    // and its 4 columns of a row of a result ([lo][second 8 columns of a panel]).
+    // and its 4 columns of a row of a result ([lo][second 8 columns of a panel][odd panel]).
     const int sw = swizzle(l32);
-    int fo[2], to[2][2], ro[2][2];
+    int fo[2], to[2][2], ro[2][2][2];
 #pragma unroll
     for (int lo = 0; lo < 2; ++lo) {
         fo[lo] = l32 * 64 + (((2 * lo + half) ^ sw) << 4);
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
-            const int l16 = lane & 15, r = 8 * half + 4 * z + (l16 >> 2);
-            to[z][lo] = (((lane >> 4) & 1) * MP + r) * 64 + (((2 * lo + ((l16 & 3) >> 1)) ^ swizzle(r)) << 4) + (l16 & 1) * 8;
-            ro[lo][z] = l32 * 64 + (((2 * lo + z) ^ sw) << 4) + 8 * half;
+            const int l16 = lane & 15, cb = (lane >> 4) & 1, r = 8 * half + 4 * z + (l16 >> 2);
+            to[z][lo] = (cb * MP + r) * 64 + (((2 * lo + ((l16 & 3) >> 1)) ^ swizzle(r, cb)) << 4) + (l16 & 1) * 8;
+#pragma unroll
+            for (int odd = 0; odd < 2; ++odd)
+                ro[lo][z][odd] = l32 * 64 + (((2 * lo + z) ^ sw ^ (odd << 1)) << 4) + 8 * half;
         }
     }
     const auto frag = [&](const uint8_t *base, int r0, int panel, int lo) {
-        return *reinterpret_cast<const half8 *>(base + (panel * MP + r0) * 64 + fo[lo]);
+        return *reinterpret_cast<const half8 *>(base + (panel * MP + r0) * 64 + (panel & 1 ? fo[lo] ^ 32 : fo[lo]));
     };
     const auto frag_t = [&](const uint8_t *base, int k0, int n0, int lo) {
         half4 h[2];
@@ -750,15 +810,15 @@ __global__ __launch_bounds__(1024) void k_muon_small(MuonTable t, MuonParams p) 
     };
     // group b of 4 columns: a result's byte without the lane's part
     const auto group_at = [&](int mt, int nt, int b) { return ((nt / 16 + (b >> 1)) * MP + mt) * 64; };
-    const auto put4 = [&](uint8_t *base, int at, int odd, const float (&v)[4]) {
+    const auto put4 = [&](uint8_t *base, int at, int b, const float (&v)[4]) {
         half4 oh, ol;
         split_fp16<4>(v, oh, ol);
-        *reinterpret_cast<half4 *>(base + at + ro[0][odd]) = oh;
-        *reinterpret_cast<half4 *>(base + at + ro[1][odd]) = ol;
+        *reinterpret_cast<half4 *>(base + at + ro[0][b & 1][b >> 1]) = oh;
+        *reinterpret_cast<half4 *>(base + at + ro[1][b & 1][b >> 1]) = ol;
     };
-    const auto get4 = [&](const uint8_t *base, int at, int odd, float (&v)[4]) {
-        const half4 h = *reinterpret_cast<const half4 *>(base + at + ro[0][odd]);
-        const half4 l = *reinterpret_cast<const half4 *>(base + at + ro[1][odd]);
+    const auto get4 = [&](const uint8_t *base, int at, int b, float (&v)[4]) {
+        const half4 h = *reinterpret_cast<const half4 *>(base + at + ro[0][b & 1][b >> 1]);
+        const half4 l = *reinterpret_cast<const half4 *>(base + at + ro[1][b & 1][b >> 1]);
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] = join_fp16(h[r], l[r]);
     };
@@ -811,7 +871,7 @@ __global__ __launch_bounds__(1024) void k_muon_small(MuonTable t, MuonParams p) 
             const int b = GB * gq + k;
 #pragma unroll
             for (int r = 0; r < 4; ++r) sq[k][r] *= kMuonScaleA / (kMuonScaleX * kMuonScaleX);
-            put4(la, group_at(gr, gc, b), b & 1, sq[k]);
+            put4(la, group_at(gr, gc, b), b, sq[k]);
         }
         __syncthreads(); // A is written
         square(la, MP / 16, sq); // ends behind a barrier: A's products are read
@@ -819,12 +879,12 @@ __global__ __launch_bounds__(1024) void k_muon_small(MuonTable t, MuonParams p) 
         for (int k = 0; k < GB; ++k) {
             const int b = GB * gq + k;
             float v[4];
-            get4(la, group_at(gr, gc, b), b & 1, v); // A until here, P from now on: the same lane's
+            get4(la, group_at(gr, gc, b), b, v); // A until here, P from now on: the same lane's
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 v[r] = __builtin_fmaf(p.b * (kMuonScaleP / kMuonScaleA), v[r],
                                       sq[k][r] * (p.c * (kMuonScaleP / (kMuonScaleA * kMuonScaleA))));
-            put4(la, group_at(gr, gc, b), b & 1, v);
+            put4(la, group_at(gr, gc, b), b, v);
         }
         __syncthreads(); // P is written
         const bool last = step == p.steps - 1;
@@ -862,11 +922,11 @@ __global__ __launch_bounds__(1024) void k_muon_small(MuonTable t, MuonParams p) 
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
                 float v[4];
-                get4(lx, group_at(mt, nt, b), b & 1, v);
+                get4(lx, group_at(mt, nt, b), b, v);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) v[r] = __builtin_fmaf(p.a, v[r], xa[k][4 * b + r] * (1.0f / kMuonScaleP));
                 if (!last) {
-                    put4(lx, group_at(mt, nt, b), b & 1, v);
+                    put4(lx, group_at(mt, nt, b), b, v);
                     continue;
                 }
                 const int m = mt + l32, n = nt + 4 * half + 8 * b;
@@ -909,24 +969,40 @@ int64_t product_tiles(int kind, const MuonEntry &e) {
     return tm * ((e.mp + BN - 1) / BN) - BM / BN * (tm * (tm - 1) / 2);
 }
 
-template<int KIND, int BM, int BN, bool SPLIT, bool PAIRS, DType W>
+template<int KIND, int BM, int BN, int KG, int ST, bool SPLIT, bool PAIRS, DType W>
 bool launch_product(MuonTable &t, const MuonStage &st, hipStream_t s) {
     const int64_t n = layout(t, [](const MuonEntry &e) { return product_tiles<BM, BN>(KIND, e); });
     if (n > INT32_MAX) return false;
     return launch_ok(
-        [&] { k_muon_product<KIND, BM, BN, SPLIT, PAIRS, W><<<dim3(static_cast<unsigned>(n)), 256, 0, s>>>(t, st); });
+        [&] { k_muon_product<KIND, BM, BN, KG, ST, SPLIT, PAIRS, W><<<dim3(static_cast<unsigned>(n)), 256 * KG, 0, s>>>(t, st); });
 }
 
 template<int KIND, bool SPLIT, bool PAIRS, DType W = DType::F32>
 bool launch_stage(MuonTable &t, const MuonStage &st, hipStream_t s) {
-    int64_t large = 0, mid = 0;
-    for (int i = 0; i < t.n; ++i) {
-        large += t.e[i].count * product_tiles<256, 128>(KIND, t.e[i]);
-        mid += t.e[i].count * product_tiles<128, 128>(KIND, t.e[i]);
+    // Tiles by an estimate of a launch's time per panel of the sum, in us, from what each took with n tiles per CU
+    // (n: between the average and the fullest CU's). fp32, 64 panels: one matrix of m = 1024, X X^T / P X, with 256 x 128:
+    // 46 / 50 us, 128 x 128: 28 / 32, 128 x 64 and two groups: 21 / 23, 64 x 64 and two: 15 / 17, and four: 13 / 15;
+    // sixteen of them 90 / 106, 80 / 123, 87 / 132, 84 / 152, 107 / 195.
+    const auto cost = [&](auto tiles_of, double per_tile, double fixed) {
+        int64_t tiles = 0;
+        for (int i = 0; i < t.n; ++i) tiles += t.e[i].count * tiles_of(t.e[i]);
+        const double n = tiles / 256.0;
+        return fixed + per_tile * (n <= 1.0 ? 1.0 : 0.5 * (n + static_cast<double>((tiles + 255) / 256)));
+    };
+    const double est[5] = {
+        cost([](const MuonEntry &e) { return product_tiles<256, 128>(KIND, e); }, 0.68, 0.12),
+        cost([](const MuonEntry &e) { return product_tiles<128, 128>(KIND, e); }, 0.36, 0.09),
+        cost([](const MuonEntry &e) { return product_tiles<128, 64>(KIND, e); }, 0.24, 0.06),
+        cost([](const MuonEntry &e) { return product_tiles<64, 64>(KIND, e); }, 0.15, 0.07),
+        cost([](const MuonEntry &e) { return product_tiles<64, 64>(KIND, e); }, 0.19, 0.00),
+    };
+    switch (std::min_element(est, est + 5) - est) {
+        case 0: return launch_product<KIND, 256, 128, 1, 3, SPLIT, PAIRS, W>(t, st, s);
+        case 1: return launch_product<KIND, 128, 128, 1, 3, SPLIT, PAIRS, W>(t, st, s);
+        case 2: return launch_product<KIND, 128, 64, 2, 3, SPLIT, PAIRS, W>(t, st, s);
+        case 3: return launch_product<KIND, 64, 64, 2, 3, SPLIT, PAIRS, W>(t, st, s);
+        default: return launch_product<KIND, 64, 64, 4, 3, SPLIT, PAIRS, W>(t, st, s);
     }
-    if (large >= 256) return launch_product<KIND, 256, 128, SPLIT, PAIRS, W>(t, st, s);
-    if (mid >= 256) return launch_product<KIND, 128, 128, SPLIT, PAIRS, W>(t, st, s);
-    return launch_product<KIND, 64, 64, SPLIT, PAIRS, W>(t, st, s);
 }
 
 } // namespace
@@ -985,10 +1061,14 @@ bool launch_muon(const MuonEntry *entries, int n, DType gt, DType wt, const Muon
     });
     if (!started) return false;
     if (t.n == 0) return true;
+    // the longest sums first, so that the launch does not end with one: by n for X X^T, by m for the others
+    MuonTable by_n = t;
+    std::stable_sort(t.e, t.e + t.n, [](const MuonEntry &x, const MuonEntry &y) { return x.mp > y.mp; });
+    std::stable_sort(by_n.e, by_n.e + by_n.n, [](const MuonEntry &x, const MuonEntry &y) { return x.np > y.np; });
     for (int k = 0; k < p.steps; ++k) {
         const MuonStage st{k & 1, p.a, p.b, p.c, p.decay};
-        bool ok = pairs ? launch_stage<kGram, true, true>(t, st, s) && launch_stage<kPoly, true, true>(t, st, s)
-                        : launch_stage<kGram, false, false>(t, st, s) && launch_stage<kPoly, true, false>(t, st, s);
+        bool ok = pairs ? launch_stage<kGram, true, true>(by_n, st, s) && launch_stage<kPoly, true, true>(t, st, s)
+                        : launch_stage<kGram, false, false>(by_n, st, s) && launch_stage<kPoly, true, false>(t, st, s);
         if (!ok) return false;
         if (k + 1 < p.steps)
             ok = pairs ? launch_stage<kApply, true, true>(t, st, s) : launch_stage<kApply, false, false>(t, st, s);

