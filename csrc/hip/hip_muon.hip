@@ -288,41 +288,31 @@ __device__ __forceinline__ uint32_t lds_offset(const uint8_t *p) {
     return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) uint8_t *)p));
 }
 
+// 16 bytes a lane from memory to LDS, 1 KB from `to` on. In assembly, so that the compiler does not make the transposing
+// reads of one tile wait for the tiles that are still on their way; the waits are this file's own (wait_tiles).
+__device__ __forceinline__ void load_to_lds(const _Float16 *from, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n"
+                 "s_nop 0\n"
+                 "global_load_lds_dwordx4 %1, off" ::"s"(to),
+                 "v"(from)
+                 : "memory", "m0");
+}
+
 // N-side fragments of kApply: at[z][s] is where this lane's part of the 4 x 16 block z of piece s lies, column block 1
-// lies YSTEP bytes further. In assembly, with its own wait: the builtin makes the compiler wait for the tiles that are
-// still on their way.
+// lies YSTEP bytes further
 template<int NT, int YSTEP>
-__device__ __forceinline__ void read_transposed(uint32_t base, const uint32_t (&at)[2][2], half8 (&f)[NT][2]) {
-    half4 h[NT][2][2];
-    if constexpr (NT == 1) {
-        asm volatile("ds_read_b64_tr_b16 %0, %4\n"
-                     "ds_read_b64_tr_b16 %1, %5\n"
-                     "ds_read_b64_tr_b16 %2, %6\n"
-                     "ds_read_b64_tr_b16 %3, %7\n"
-                     "s_waitcnt lgkmcnt(0)"
-                     : "=&v"(h[0][0][0]), "=&v"(h[0][0][1]), "=&v"(h[0][1][0]), "=&v"(h[0][1][1])
-                     : "v"(base + at[0][0]), "v"(base + at[0][1]), "v"(base + at[1][0]), "v"(base + at[1][1])
-                     : "memory");
-    } else {
-        static_assert(NT == 2);
-        asm volatile("ds_read_b64_tr_b16 %0, %8\n"
-                     "ds_read_b64_tr_b16 %1, %9\n"
-                     "ds_read_b64_tr_b16 %2, %10\n"
-                     "ds_read_b64_tr_b16 %3, %11\n"
-                     "ds_read_b64_tr_b16 %4, %8 offset:%12\n"
-                     "ds_read_b64_tr_b16 %5, %9 offset:%12\n"
-                     "ds_read_b64_tr_b16 %6, %10 offset:%12\n"
-                     "ds_read_b64_tr_b16 %7, %11 offset:%12\n"
-                     "s_waitcnt lgkmcnt(0)"
-                     : "=&v"(h[0][0][0]), "=&v"(h[0][0][1]), "=&v"(h[0][1][0]), "=&v"(h[0][1][1]), "=&v"(h[1][0][0]),
-                       "=&v"(h[1][0][1]), "=&v"(h[1][1][0]), "=&v"(h[1][1][1])
-                     : "v"(base + at[0][0]), "v"(base + at[0][1]), "v"(base + at[1][0]), "v"(base + at[1][1]), "n"(YSTEP)
-                     : "memory");
-    }
+__device__ __forceinline__ void read_transposed(const uint8_t *base, const uint32_t (&at)[2][2], half8 (&f)[NT][2]) {
 #pragma unroll
     for (int y = 0; y < NT; ++y)
 #pragma unroll
-        for (int s = 0; s < 2; ++s) f[y][s] = __builtin_shufflevector(h[y][0][s], h[y][1][s], 0, 1, 2, 3, 4, 5, 6, 7);
+        for (int s = 0; s < 2; ++s) {
+            half4 h[2];
+#pragma unroll
+            for (int z = 0; z < 2; ++z)
+                h[z] = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                     (__attribute__((address_space(3))) short4v *)(base + at[z][s] + y * YSTEP)));
+            f[y][s] = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        }
 }
 
 // 16-byte pieces of a panel's 64-byte rows trade places in LDS: a fragment's 16-byte reads are served 16 rows at a time
@@ -331,9 +321,11 @@ __device__ __forceinline__ void read_transposed(uint32_t base, const uint32_t (&
 __device__ __forceinline__ int swizzle(int r) { return (r >> 2) & 3; }
 __device__ __forceinline__ int swizzle(int r, int panel) { return swizzle(r) ^ ((panel & 1) << 1); }
 
-// Work item of this workgroup. Workgroups go to the 8 chiplets in turn; each gets runs of kRun neighbouring tiles, which
-// share operands in its L2, and the runs advance together, because the items are sorted by falling length.
-constexpr int kRun = 32;
+// Work item of this workgroup. Workgroups go to the 8 chiplets in turn; each gets runs of neighbouring tiles, which share
+// operands in its L2, and the runs advance together, because the items are sorted by falling length. What the L2s miss
+// is what bounds these kernels apart from their products. A run of P X is kBand rows of tiles and as many columns.
+constexpr int kBand = 8;
+template<int kRun>
 __device__ __forceinline__ int place_of_block() {
     const int b = blockIdx.x, n = gridDim.x, window = 8 * kRun;
     const int base = b / window * window, run = n - base < window ? (n - base) / 8 : kRun;
@@ -346,33 +338,34 @@ __device__ __forceinline__ int place_of_block() {
 // fragments are transposed on their way out of LDS. Both sides travel straight to LDS, a panel of the sum at a time.
 // SPLIT: three products of the parts. PAIRS: X and P lie in pairs. The MFMA's first operand is the N side: a lane then
 // holds 4 neighbouring columns of one row.
-// KG groups of four waves take the panels in turn and add their sums up at the end: with few tiles this fills the CUs.
+// WV waves share a tile, two along m. KG groups of them take the panels in turn and add their sums up at the end: with few tiles this fills the CUs.
 // Of ST panels in a group's part of LDS one is multiplied, the others are on their way.
-template<int KIND, int BM, int BN, int KG, int ST, bool SPLIT, bool PAIRS, DType W>
-__global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void k_muon_product(MuonTable t, MuonStage st) {
-    constexpr int WM = BM / 2, WN = BN / 2, MT = WM / 32, NT = WN / 32;
+template<int KIND, int BM, int BN, int WV, int KG, int ST, bool SPLIT, bool PAIRS, DType W>
+__global__ __launch_bounds__(64 * WV * KG, KG == 1 ? 2 : 4) void k_muon_product(MuonTable t, MuonStage st) {
+    constexpr int WM = BM / 2, WN = BN / (WV / 2), MT = WM / 32, NT = WN / 32;
     constexpr int BK = SPLIT ? 16 : 32; // columns of a panel, the step along the sum
     constexpr bool NN = KIND == kApply || KIND == kFinal;
+    constexpr bool AHEAD = MT * NT <= 4; // registers for two tiles' fragments
     constexpr int kTile = (BM + BN) * 64;
     constexpr int kSlice = 32 * (WN + 4) * 4; // 32 rows of a wave's results, padded against bank conflicts
-    constexpr int kLds = KG * (ST * kTile > 4 * kSlice ? ST * kTile : 4 * kSlice);
+    constexpr int kLds = KG * (ST * kTile > WV * kSlice ? ST * kTile : WV * kSlice);
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
 
-    const int blk = place_of_block();
+    const int blk = place_of_block<NN ? kBand * kBand : 32>();
     const int i = entry_of(t, blk);
     const MuonEntry &e = t.e[i];
     const int rows = e.mp;
     const int tm = (rows + BM - 1) / BM, tn = ((NN ? e.np : rows) + BN - 1) / BN;
+    constexpr int R = BM / BN;
+    const int b = blk - t.first[i];
     int ti, tj, which;
     if constexpr (NN) {
-        const int b = blk - t.first[i];
         which = b / (tm * tn);
-        ti = b % (tm * tn) % tm;
-        tj = b % (tm * tn) / tm;
+        const int rest = b % (tm * tn), band = rest / (kBand * tn) * kBand, h = tm - band < kBand ? tm - band : kBand;
+        ti = band + (rest - band * tn) % h;
+        tj = (rest - band * tn) / h;
     } else { // tiles that reach the diagonal or lie above it
-        constexpr int R = BM / BN;
         const int tiles = tm * tn - R * (tm * (tm - 1) / 2);
-        const int b = blk - t.first[i];
         which = b / tiles;
         int rest = b % tiles;
         ti = 0;
@@ -386,9 +379,10 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void k_muon_product(Muon
     const _Float16 *ms = KIND == kGram ? x : KIND == kPoly ? q.a : q.p;
     const _Float16 *ns = KIND == kPoly ? q.a : x;
 
-    const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) & 3, group = threadIdx.x >> 8;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) % WV),
+              group = __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * WV));
     // source of each 16-byte piece this lane brings to LDS; rows and panels past the matrix repeat its last ones
-    constexpr int MI = BM / 64, NI = BN / 64;
+    constexpr int MI = BM / (16 * WV), NI = BN / (16 * WV);
     const _Float16 *mp[MI], *np[NI];
     const int lrow = lane >> 2;
     const int lpiece = (lane & 3) ^ swizzle(lrow);
@@ -412,19 +406,15 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void k_muon_product(Muon
     const size_t mstep = static_cast<size_t>(rows) * 32 * KG, nstep = NN ? BK * 32 * KG : mstep;
     uint8_t *mine = lds + group * ST * kTile;
     const auto fetch = [&](int buf) {
-        uint8_t *to = mine + buf * kTile;
+        const uint32_t to = __builtin_amdgcn_readfirstlane(lds_offset(mine + buf * kTile));
 #pragma unroll
         for (int k = 0; k < MI; ++k) {
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)mp[k],
-                                             (__attribute__((address_space(3))) void *)(to + (wave * MI + k) * 1024), 16,
-                                             0, 0);
+            load_to_lds(mp[k], to + (wave * MI + k) * 1024);
             mp[k] += mstep;
         }
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
-            __builtin_amdgcn_global_load_lds(
-                (const __attribute__((address_space(1))) void *)np[k],
-                (__attribute__((address_space(3))) void *)(to + BM * 64 + (wave * NI + k) * 1024), 16, 0, 0);
+            load_to_lds(np[k], to + BM * 64 + (wave * NI + k) * 1024);
             np[k] += nstep;
         }
     };
@@ -469,17 +459,9 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void k_muon_product(Muon
     }
     float16v acc[NT][MT] = {};
     const int panels = K / BK, rounds = (panels + KG - 1) / KG, steps = (panels - group + KG - 1) / KG; // this group's
-#pragma unroll
-    for (int k = 0; k < ST - 1; ++k)
-        if (k < steps) fetch(k);
-    for (int k = 0, buf = 0, to = ST - 1; k < rounds; ++k) {
-        const int later = steps - 1 - k; // tiles behind this one
-        wait_tiles<MI + NI, ST - 1>(later < ST - 2 ? (later > 0 ? later : 0) : ST - 2);
-        __builtin_amdgcn_s_barrier(); // tile k has landed for every wave, and all are done with tile k - 1
-        asm volatile("" ::: "memory");
-        if (KG > 1 && k >= steps) break; // the last round, without a panel for this group
+    const auto read = [&](int buf, half8 (&mf)[MT][2], half8 (&nf)[NT][2]) {
+        // two pieces of 16 of the sum: hi and lo of one, or both of 32
         const uint8_t *ml = mine + buf * kTile, *nl = ml + BM * 64;
-        half8 mf[MT][2], nf[NT][2]; // two pieces of 16 of the sum: hi and lo of one, or both of 32
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             const int at = l32 * 64 + (((2 * s + half) ^ swizzle(l32)) << 4);
@@ -490,10 +472,9 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void k_muon_product(Muon
                 for (int y = 0; y < NT; ++y) nf[y][s] = *reinterpret_cast<const half8 *>(nl + (wn + y * 32) * 64 + at);
             }
         }
-        if constexpr (NN) read_transposed<NT, 32 / BK * BK * 64>(lds_offset(nl), tr, nf);
-        if (k + ST - 1 < steps) fetch(to); // over tile k - 1
-        buf = buf == ST - 1 ? 0 : buf + 1;
-        to = to == ST - 1 ? 0 : to + 1;
+        if constexpr (NN) read_transposed<NT, 32 / BK * BK * 64>(nl, tr, nf);
+    };
+    const auto multiply = [&](const half8 (&mf)[MT][2], const half8 (&nf)[NT][2]) {
         const auto mul = [&](int sn, int sm) {
 #pragma unroll
             for (int y = 0; y < NT; ++y)
@@ -508,6 +489,49 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void k_muon_product(Muon
         } else {
             mul(1, 1);
         }
+    };
+    if constexpr (AHEAD) {
+        // the next tile's fragments are read while this one's are multiplied
+        half8 mf[2][MT][2], nf[2][NT][2];
+#pragma unroll
+        for (int k = 0; k < ST; ++k)
+            if (k < steps) fetch(k);
+        wait_tiles<MI + NI, ST>(steps - 1 < ST - 1 ? (steps > 1 ? steps - 1 : 0) : ST - 1);
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (steps > 0) read(0, mf[0], nf[0]);
+        int buf = 0;
+        const auto round = [&](int k, int set) {
+            const int next = buf == ST - 1 ? 0 : buf + 1, later = steps - 2 - k; // tiles behind the next one
+            wait_tiles<MI + NI, ST - 1>(later < ST - 2 ? (later > 0 ? later : 0) : ST - 2);
+            __builtin_amdgcn_s_barrier(); // tile k + 1 has landed for every wave, and all have read tile k
+            asm volatile("" ::: "memory");
+            if (k + 1 < steps) read(next, mf[set ^ 1], nf[set ^ 1]);
+            if (k + ST < steps) fetch(buf);
+            if (k < steps) multiply(mf[set], nf[set]);
+            buf = next;
+        };
+        for (int k = 0; k < rounds; k += 2) {
+            round(k, 0);
+            if (k + 1 < rounds) round(k + 1, 1);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < ST - 1; ++k)
+            if (k < steps) fetch(k);
+        for (int k = 0, buf = 0, to = ST - 1; k < rounds; ++k) {
+            const int later = steps - 1 - k; // tiles behind this one
+            wait_tiles<MI + NI, ST - 1>(later < ST - 2 ? (later > 0 ? later : 0) : ST - 2);
+            __builtin_amdgcn_s_barrier(); // tile k has landed for every wave, and all are done with tile k - 1
+            asm volatile("" ::: "memory");
+            if (KG > 1 && k >= steps) break; // the last round, without a panel for this group
+            half8 mf[MT][2], nf[NT][2];
+            read(buf, mf, nf);
+            if (k + ST - 1 < steps) fetch(to); // over tile k - 1
+            buf = buf == ST - 1 ? 0 : buf + 1;
+            to = to == ST - 1 ? 0 : to + 1;
+            multiply(mf, nf);
+        }
     }
     __syncthreads(); // the tiles' memory now carries results
 
@@ -518,7 +542,7 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void k_muon_product(Muon
     const int small = flip ? e.cols : e.rows, large = flip ? e.rows : e.cols;
     constexpr int kPitch = WN + 4;
     // a wave's slice of its own sums, the first group's (the whole sum's), and what orders accesses to them
-    float *own = reinterpret_cast<float *>(lds + (group * 4 + wave) * kSlice);
+    float *own = reinterpret_cast<float *>(lds + (group * WV + wave) * kSlice);
     float *slice = reinterpret_cast<float *>(lds + wave * kSlice);
     const auto sync = [] {
         if constexpr (KG == 1)
@@ -573,7 +597,7 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void k_muon_product(Muon
             *reinterpret_cast<float4 *>(v + 4) = *reinterpret_cast<const float4 *>(slice + r * kPitch + c + 4);
 #pragma unroll
             for (int j = 1; j < KG; ++j) {
-                const float *other = slice + j * kSlice + r * kPitch + c; // 4 slices a group, 4 bytes an element
+                const float *other = slice + j * WV * (kSlice / 4) + r * kPitch + c;
 #pragma unroll
                 for (int k = 0; k < 8; ++k) v[k] += other[k];
             }
@@ -969,39 +993,42 @@ int64_t product_tiles(int kind, const MuonEntry &e) {
     return tm * ((e.mp + BN - 1) / BN) - BM / BN * (tm * (tm - 1) / 2);
 }
 
-template<int KIND, int BM, int BN, int KG, int ST, bool SPLIT, bool PAIRS, DType W>
+template<int KIND, int BM, int BN, int WV, int KG, int ST, bool SPLIT, bool PAIRS, DType W>
 bool launch_product(MuonTable &t, const MuonStage &st, hipStream_t s) {
     const int64_t n = layout(t, [](const MuonEntry &e) { return product_tiles<BM, BN>(KIND, e); });
     if (n > INT32_MAX) return false;
     return launch_ok(
-        [&] { k_muon_product<KIND, BM, BN, KG, ST, SPLIT, PAIRS, W><<<dim3(static_cast<unsigned>(n)), 256 * KG, 0, s>>>(t, st); });
+        [&] { k_muon_product<KIND, BM, BN, WV, KG, ST, SPLIT, PAIRS, W><<<dim3(static_cast<unsigned>(n)), 64 * WV * KG, 0, s>>>(t, st); });
 }
 
 template<int KIND, bool SPLIT, bool PAIRS, DType W = DType::F32>
 bool launch_stage(MuonTable &t, const MuonStage &st, hipStream_t s) {
-    // Tiles by an estimate of a launch's time per panel of the sum, in us, from what each took with n tiles per CU
-    // (n: between the average and the fullest CU's). fp32, 64 panels: one matrix of m = 1024, X X^T / P X, with 256 x 128:
-    // 46 / 50 us, 128 x 128: 28 / 32, 128 x 64 and two groups: 21 / 23, 64 x 64 and two: 15 / 17, and four: 13 / 15;
-    // sixteen of them 90 / 106, 80 / 123, 87 / 132, 84 / 152, 107 / 195.
-    const auto cost = [&](auto tiles_of, double per_tile, double fixed) {
+    // Tiles by an estimate of a launch's time per panel of the sum, in us, fitted to what each took with n tiles per CU
+    // (n between the average and the fullest CU's, or that of the fullest where only one fits). In us, fp32, X X^T / P X,
+    // for 256 x 128, 128 x 128, 128 x 64, 64 x 64 by two groups of waves and by four:
+    //   1 x 1024 x 1024     45 / 48     29 / 32     22 / 24     14 / 16     13 / 15
+    //   12 x 768 x 768      42 / 48     31 / 41     29 / 45     30 / 54     40 / 70
+    //   4 x 1024 x 4096    157 / 102   103 / 106    93 / 114    89 / 157    99 / 188
+    //   2 x 4096 x 4096    491 / 670   435 / 724   471 / 830   603 / 1022  649 / 1137
+    const auto cost = [&](auto tiles_of, double per_tile, double fixed, bool one_fits = false) {
         int64_t tiles = 0;
         for (int i = 0; i < t.n; ++i) tiles += t.e[i].count * tiles_of(t.e[i]);
-        const double n = tiles / 256.0;
-        return fixed + per_tile * (n <= 1.0 ? 1.0 : 0.5 * (n + static_cast<double>((tiles + 255) / 256)));
+        const double average = tiles / 256.0, fullest = static_cast<double>((tiles + 255) / 256);
+        return fixed + per_tile * (one_fits ? fullest : average <= 1.0 ? 1.0 : 0.5 * (average + fullest));
     };
     const double est[5] = {
-        cost([](const MuonEntry &e) { return product_tiles<256, 128>(KIND, e); }, 0.68, 0.12),
-        cost([](const MuonEntry &e) { return product_tiles<128, 128>(KIND, e); }, 0.36, 0.09),
-        cost([](const MuonEntry &e) { return product_tiles<128, 64>(KIND, e); }, 0.24, 0.06),
-        cost([](const MuonEntry &e) { return product_tiles<64, 64>(KIND, e); }, 0.15, 0.07),
-        cost([](const MuonEntry &e) { return product_tiles<64, 64>(KIND, e); }, 0.19, 0.00),
+        cost([](const MuonEntry &e) { return product_tiles<256, 128>(KIND, e); }, 0.62, 0.21),
+        cost([](const MuonEntry &e) { return product_tiles<128, 128>(KIND, e); }, 0.33, 0.16),
+        cost([](const MuonEntry &e) { return product_tiles<128, 64>(KIND, e); }, 0.22, 0.10),
+        cost([](const MuonEntry &e) { return product_tiles<64, 64>(KIND, e); }, 0.122, 0.12),
+        cost([](const MuonEntry &e) { return product_tiles<64, 64>(KIND, e); }, 0.20, 0.00, true),
     };
     switch (std::min_element(est, est + 5) - est) {
-        case 0: return launch_product<KIND, 256, 128, 1, 3, SPLIT, PAIRS, W>(t, st, s);
-        case 1: return launch_product<KIND, 128, 128, 1, 3, SPLIT, PAIRS, W>(t, st, s);
-        case 2: return launch_product<KIND, 128, 64, 2, 3, SPLIT, PAIRS, W>(t, st, s);
-        case 3: return launch_product<KIND, 64, 64, 2, 3, SPLIT, PAIRS, W>(t, st, s);
-        default: return launch_product<KIND, 64, 64, 4, 3, SPLIT, PAIRS, W>(t, st, s);
+        case 0: return launch_product<KIND, 256, 128, 4, 1, 3, SPLIT, PAIRS, W>(t, st, s);
+        case 1: return launch_product<KIND, 128, 128, 4, 1, 3, SPLIT, PAIRS, W>(t, st, s);
+        case 2: return launch_product<KIND, 128, 64, 4, 1, 3, SPLIT, PAIRS, W>(t, st, s);
+        case 3: return launch_product<KIND, 64, 64, 4, 2, 3, SPLIT, PAIRS, W>(t, st, s);
+        default: return launch_product<KIND, 64, 64, 4, 4, 3, SPLIT, PAIRS, W>(t, st, s);
     }
 }
 
