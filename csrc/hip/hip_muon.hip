@@ -6,9 +6,10 @@
 // a X + P X, whose last pass updates the caller's parameters instead of writing X. No atomics and a fixed order of
 // every sum: equal calls give equal bits, which the peers of a run rely on.
 //
-// The products of the 16-bit types: where the result is bf16 (8 bits), A and P X use the hi parts alone (11 bits) and
-// only A A, the cheapest, all three; the term a X always has both parts, so small singular values, which the steps
-// amplify up to a^steps, keep their precision. Other results use three products everywhere, the error of fp32 products.
+// The products of the 16-bit types: where the result is bf16 (8 bits) and the matrices are not small (launch_muon), A
+// and P X use the hi parts alone (11 bits) and only A A, the cheapest, all three; the term a X always has both parts, so
+// small singular values, which the steps amplify up to a^steps, keep their precision. Otherwise three products
+// everywhere, the error of fp32 products.
 #include <algorithm>
 
 #include "dispatch.hpp"
@@ -1058,7 +1059,13 @@ bool launch_muon(const MuonEntry *entries, int n, DType gt, DType wt, const Muon
         to.e[to.n++] = entries[i];
         if (&to == &narrow) np = np > entries[i].np ? np : entries[i].np;
     }
-    const bool pairs = wt != DType::BF16; // three products everywhere
+    // Three products everywhere: where the result has more bits than one product, and for small matrices, whose sums are
+    // too short to average the roundings of one product out (sides below 200: up to 1.46 times the error of the bf16
+    // result's own rounding, against 1.00; 1.1 to 1.36 from 320 to 2048). In us, one product / three: 12 x 256 x 256
+    // 102 / 116, 12 x 256 x 1024 136 / 170, 48 x 256 x 1024 242 / 339; above, 12 x 768 x 768 343 / 495.
+    int largest = 0;
+    for (int i = 0; i < t.n; ++i) largest = std::max(largest, t.e[i].mp);
+    const bool pairs = wt != DType::BF16 || largest <= 256;
     const auto with_grad = [&](auto &&f) {
         switch (gt) {
             case DType::F32: return f(std::integral_constant<DType, DType::F32>{});
@@ -1104,7 +1111,8 @@ bool launch_muon(const MuonEntry *entries, int n, DType gt, DType wt, const Muon
         else if (wt == DType::F16)
             ok = launch_stage<kFinal, true, true, DType::F16>(t, st, s);
         else
-            ok = launch_stage<kFinal, false, false, DType::BF16>(t, st, s);
+            ok = pairs ? launch_stage<kFinal, true, true, DType::BF16>(t, st, s)
+                       : launch_stage<kFinal, false, false, DType::BF16>(t, st, s);
         if (!ok) return false;
     }
     return true;
