@@ -269,7 +269,7 @@ PCCLX_EXPORT int pcclxTokenLogprobs(const void *logits, int64_t row_stride, int6
     DeviceBackend *be = device_backend();
     if (!be) return -1;
     if (rows < 0 || rows > INT32_MAX || vocab < 1 || vocab > INT32_MAX || top_k < 0 ||
-        top_k > kernels::kMaxTopLogprobs || top_k > vocab)
+        top_k > kernels::kMaxTopLogprobs || top_k > vocab || (rows && (!logits || !targets)))
         return -2;
     const kernels::LogprobArgs a{logits,  row_stride, rows,  vocab,       targets,  ignore_index,
                                  top_k,   logprob,    entropy, stats, top_logprob, top_index};
@@ -285,7 +285,7 @@ PCCLX_EXPORT int pcclxTokenLogprobsGrad(const void *logits, int64_t row_stride, 
     DeviceBackend *be = device_backend();
     if (!be) return -1;
     if (rows < 0 || rows > INT32_MAX || vocab < 1 || vocab > INT32_MAX || top_k < 0 ||
-        top_k > kernels::kMaxTopLogprobs || top_k > vocab)
+        top_k > kernels::kMaxTopLogprobs || top_k > vocab || (rows && (!logits || !targets || !stats || !d_logits)))
         return -2;
     kernels::LogprobGradArgs g;
     g.fwd = {logits, row_stride, rows, vocab, targets, ignore_index, top_k, nullptr, nullptr,
@@ -367,6 +367,7 @@ PCCLX_EXPORT int pcclxMuon(int n, const int64_t *shapes, const void *const *g, i
             e.alpha = alpha ? alpha[i] : 0.0f;
             const size_t elems = static_cast<size_t>(e.count) * e.rows * e.cols;
             if (elems == 0) continue;
+            if (!e.g || !e.w || (mom && !e.mom)) return -2; // a tensor without storage of its own
             const auto span = [&](const void *p, size_t es, bool written) {
                 const auto from = reinterpret_cast<uintptr_t>(p);
                 spans.push_back({from, from + elems * es, written});

@@ -34,6 +34,9 @@ def parser(desc: str) -> argparse.ArgumentParser:
     ap.add_argument("--max-iters", type=int, default=100)
     ap.add_argument("--lr", type=float, default=6e-4)
     ap.add_argument("--min-lr", type=float, default=6e-5)
+    ap.add_argument("--optimizer", default="adamw", choices=["adamw", "muon"])
+    ap.add_argument("--fused-loss", action="store_true",
+                    help="loss from the logits in their own type, in one pass (no fp32 copy)")
     ap.add_argument("--warmup-iters", type=int, default=10)
     ap.add_argument("--weight-decay", type=float, default=0.1)
     ap.add_argument("--grad-clip", type=float, default=1.0)
@@ -54,9 +57,9 @@ def device_of(a) -> torch.device:
 
 def build(a, device: torch.device):
     torch.manual_seed(a.seed)
-    cfg = GPTConfig(**PRESETS[a.preset])
+    cfg = GPTConfig(**PRESETS[a.preset], fused_loss=a.fused_loss)
     model = GPT(cfg).to(device)
-    opt = model.configure_optimizers(a.weight_decay, a.lr, (0.9, 0.95), device.type)
+    opt = model.configure_optimizers(a.weight_decay, a.lr, (0.9, 0.95), device.type, a.optimizer)
     data = TokenStream(a.data, vocab_size=cfg.vocab_size, seed=a.seed + int(os.environ.get("RANK", "0")) + os.getpid())
     ctx = torch.autocast(device_type=device.type, dtype=torch.bfloat16) if a.dtype == "bfloat16" else nullcontext()
     return cfg, model, opt, data, ctx

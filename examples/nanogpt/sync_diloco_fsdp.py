@@ -31,6 +31,8 @@ def main():
     ap.add_argument("--outer-lr", type=float, default=0.7)
     ap.add_argument("--nodes", type=int, default=2, help="expected number of nodes (peers per peer group)")
     a = ap.parse_args()
+    if a.optimizer != "adamw":
+        ap.error("--optimizer muon needs whole matrices, FSDP2 shards them")
     device = device_of(a)
     if device.type == "cuda":
         torch.cuda.set_device(device)

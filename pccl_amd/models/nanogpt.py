@@ -6,7 +6,11 @@ projections, AdamW param groups with/without weight decay, 6N+12LHQT FLOP estima
 
 * attention is ``scaled_dot_product_attention`` (PyTorch-ROCm dispatches it to its CK/AOTriton flash kernels);
 * training runs in bf16 autocast (MFU priced against the 2.5 PFLOP/s dense bf16 peak of one MI355X);
-* AdamW uses the fused multi-tensor implementation when parameters live on the GPU.
+* AdamW uses the fused multi-tensor implementation when parameters live on the GPU; Muon, for the matrices of the
+  blocks, is :class:`pccl_amd.parallel.Muon`;
+* ``fused_loss`` takes the loss from the logits in their own type (:func:`pccl_amd.ops.token_logprobs`): no fp32 copy of
+  (tokens, vocabulary), one pass forward and one backward. :meth:`GPT.score` and ``generate``'s log probabilities use
+  the same kernel.
 """
 from __future__ import annotations
 
@@ -17,6 +21,9 @@ from typing import Optional, Tuple
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from ..ops.logprobs import TokenLogprobs, token_logprobs
+from ..parallel.muon import Muon
 
 MI355X_BF16_DENSE_FLOPS = 2.5e15
 
@@ -30,6 +37,7 @@ class GPTConfig:
     n_embd: int = 768
     dropout: float = 0.0
     bias: bool = True
+    fused_loss: bool = False
 
 
 class Block(nn.Module):
@@ -86,8 +94,7 @@ class GPT(nn.Module):
         n = sum(p.numel() for p in self.parameters())
         return n - self.wpe.weight.numel() if non_embedding else n
 
-    def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None
-                ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    def logits(self, idx: torch.Tensor) -> torch.Tensor:
         b, t = idx.shape
         assert t <= self.config.block_size, f"sequence {t} > block size {self.config.block_size}"
         pos = torch.arange(t, device=idx.device)
@@ -95,9 +102,16 @@ class GPT(nn.Module):
         for blk in self.h:
             x = blk(x)
         x = self.ln_f(x)
-        logits = F.linear(x, self.wte.weight)  # tied lm head
+        return F.linear(x, self.wte.weight)  # tied lm head
+
+    def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None
+                ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+        logits = self.logits(idx)
         if targets is None:
             return logits[:, -1:, :], None
+        if self.config.fused_loss:
+            logprob = token_logprobs(logits.view(-1, logits.size(-1)), targets.reshape(-1), ignore_index=-1).logprob
+            return logits, -logprob.sum() / (targets != -1).sum()
         loss = F.cross_entropy(logits.float().view(-1, logits.size(-1)), targets.view(-1), ignore_index=-1)
         return logits, loss
 
@@ -107,8 +121,20 @@ class GPT(nn.Module):
         self.wpe.weight = nn.Parameter(self.wpe.weight[:block_size].detach().clone())
 
     def configure_optimizers(self, weight_decay: float, learning_rate: float, betas=(0.9, 0.95),
-                             device_type: str = "cuda") -> torch.optim.AdamW:
+                             device_type: str = "cuda", optimizer: str = "adamw") -> torch.optim.Optimizer:
+        """``optimizer``: "adamw", or "muon" for the matrices of the blocks with AdamW for the embeddings, biases and
+        norms; one learning rate and weight decay serve both."""
         params = [p for p in self.parameters() if p.requires_grad]
+        if optimizer == "muon":
+            matrices = [p for p in self.h.parameters() if p.requires_grad and p.dim() == 2]
+            hidden = set(matrices)
+            rest = [p for p in params if p not in hidden]
+            groups = [{"params": [p for p in rest if p.dim() >= 2], "weight_decay": weight_decay},
+                      {"params": [p for p in rest if p.dim() < 2], "weight_decay": 0.0}]
+            return Muon(matrices, [g for g in groups if g["params"]], lr=learning_rate, weight_decay=weight_decay,
+                        betas=betas, fused=device_type == "cuda")
+        if optimizer != "adamw":
+            raise ValueError(f"optimizer must be 'adamw' or 'muon', got {optimizer!r}")
         decay = [p for p in params if p.dim() >= 2]
         no_decay = [p for p in params if p.dim() < 2]
         groups = [{"params": decay, "weight_decay": weight_decay}, {"params": no_decay, "weight_decay": 0.0}]
@@ -122,14 +148,29 @@ class GPT(nn.Module):
         return self.flops_per_token() * tokens_per_iter / dt / peak
 
     @torch.no_grad()
+    def score(self, idx: torch.Tensor, targets: torch.Tensor, top_k: int = 0) -> TokenLogprobs:
+        """Log probability of ``targets[b, t]`` after ``idx[b, :t + 1]`` (0 where it is -1), the entropy of the model's
+        distribution there and its ``top_k`` alternatives."""
+        return token_logprobs(self.logits(idx), targets, top_k=top_k, ignore_index=-1)
+
+    @torch.no_grad()
     def generate(self, idx: torch.Tensor, max_new_tokens: int, temperature: float = 1.0,
-                 top_k: Optional[int] = None) -> torch.Tensor:
+                 top_k: Optional[int] = None, return_logprobs: bool = False):
+        """``idx`` with ``max_new_tokens`` sampled tokens behind it; with ``return_logprobs`` also their log
+        probabilities (fp32, [batch, max_new_tokens]) under the model, before ``temperature`` and ``top_k``."""
+        logprobs = []
         for _ in range(max_new_tokens):
             ctx = idx if idx.size(1) <= self.config.block_size else idx[:, -self.config.block_size:]
-            logits, _ = self(ctx)
-            logits = logits[:, -1, :] / temperature
+            raw, _ = self(ctx)
+            raw = raw[:, -1, :]
+            logits = raw / temperature
             if top_k is not None:
                 v, _ = torch.topk(logits, min(top_k, logits.size(-1)))
                 logits[logits < v[:, [-1]]] = -float("inf")
-            idx = torch.cat((idx, torch.multinomial(F.softmax(logits, dim=-1), num_samples=1)), dim=1)
+            token = torch.multinomial(F.softmax(logits, dim=-1), num_samples=1)
+            if return_logprobs:
+                logprobs.append(token_logprobs(raw, token[:, 0]).logprob)
+            idx = torch.cat((idx, token), dim=1)
+        if return_logprobs:
+            return idx, torch.stack(logprobs, dim=1) if logprobs else idx.new_zeros((idx.size(0), 0), dtype=torch.float32)
         return idx

@@ -175,7 +175,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top_k: int = 
     * a row with a NaN or ``+inf`` has NaN results and gradients.
 
     ``logprob``, ``entropy`` and ``top_logprob`` are differentiable (once) with respect to ``logits``; the call and its
-    backward only queue kernels, so both may be captured into a graph.
+    backward only queue kernels, so both may be captured into a graph. (Before a backward pass is captured, drop the
+    results of eager calls on the same leaves: torch ends the process when their graph is still alive.)
     """
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"token_logprobs: logits need a vocabulary dimension, got shape {tuple(logits.shape)}")

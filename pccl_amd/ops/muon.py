@@ -126,6 +126,18 @@ def _shape_factor(rows: int, cols: int, adjust_lr: str) -> float:
     raise ValueError(f"muon_step: adjust_lr must be 'original', 'match_rms_adamw' or 'none', got {adjust_lr!r}")
 
 
+def check_muon(what: str, lr: float, weight_decay: float, momentum: float, steps: int,
+               coefficients: Tuple[float, ...], eps: float, adjust_lr: str) -> None:
+    _check_coefficients(coefficients, steps)
+    if not eps > 0 or not math.isfinite(eps):
+        raise ValueError(f"{what}: eps must be positive, got {eps}")
+    if not 0.0 <= momentum <= 1.0:
+        raise ValueError(f"{what}: momentum must be in 0..1, got {momentum}")
+    if not (math.isfinite(lr) and math.isfinite(weight_decay)):
+        raise ValueError(f"{what}: lr {lr} and weight_decay {weight_decay} must be finite")
+    _shape_factor(1, 1, adjust_lr)
+
+
 def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
               momentum_buffers: Sequence[torch.Tensor], *, lr: float, weight_decay: float = 0.1,
               momentum: float = 0.95, nesterov: bool = True, steps: int = 5,
@@ -143,17 +155,10 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     memory with another (a parameter listed twice is refused). Equal calls give equal bits on every peer.
     """
     coefficients, steps = tuple(coefficients), int(steps)
-    _check_coefficients(coefficients, steps)
+    check_muon("muon_step", lr, weight_decay, momentum, steps, coefficients, eps, adjust_lr)
     if not len(params) == len(grads) == len(momentum_buffers):
         raise ValueError(f"muon_step: {len(params)} parameters, {len(grads)} gradients and {len(momentum_buffers)} "
                          "momentum buffers")
-    if not eps > 0 or not math.isfinite(eps):
-        raise ValueError(f"muon_step: eps must be positive, got {eps}")
-    if not 0.0 <= momentum <= 1.0:
-        raise ValueError(f"muon_step: momentum must be in 0..1, got {momentum}")
-    if not (math.isfinite(lr) and math.isfinite(weight_decay)):
-        raise ValueError(f"muon_step: lr {lr} and weight_decay {weight_decay} must be finite")
-    _shape_factor(1, 1, adjust_lr)
     if not params:
         return
     device, wtype, gtype = params[0].device, params[0].dtype, grads[0].dtype
