@@ -10,6 +10,8 @@
 // where it first stood, and 64 groups of threads the best of these. Ordered by (value, earlier block), the k-th best of
 // the 64 pairs bounds the k best elements from below -- each of the k better groups has an element that beats everything
 // in a group behind it -- so only threads of k groups have their elements looked at again.
+#include <algorithm>
+
 #include "dispatch.hpp"
 #include "launchers.hpp"
 
@@ -25,6 +27,7 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kNegInf = -__builtin_inff();
 constexpr int kUnroll = 4;      // 16-byte loads in flight per thread
 constexpr int kCandidates = 1024;
+constexpr int64_t kRowsPerLaunch = 1 << 22; // a launch has fewer than 2^32 threads
 
 // storage types with the hardware conversions (round to nearest even)
 struct LF32 {
@@ -350,6 +353,19 @@ __global__ __launch_bounds__(T) void k_token_logprob_grad(LogprobGradArgs g, int
     }
 }
 
+// the n rows from r0 on
+static LogprobArgs rows_of(LogprobArgs a, int64_t r0, int64_t n, size_t esize) {
+    a.logits = static_cast<const uint8_t *>(a.logits) + esize * a.row_stride * r0;
+    a.rows = n;
+    a.targets += r0;
+    a.stats += 3 * r0;
+    if (a.logprob) a.logprob += r0;
+    if (a.entropy) a.entropy += r0;
+    if (a.top_logprob) a.top_logprob += r0 * a.top_k;
+    if (a.top_index) a.top_index += r0 * a.top_k;
+    return a;
+}
+
 template<typename F>
 static bool with_logit(DType t, F &&f) {
     switch (t) {
@@ -362,6 +378,11 @@ static bool with_logit(DType t, F &&f) {
 
 bool launch_token_logprobs(const LogprobArgs &a, DType t, hipStream_t st) {
     if (a.rows == 0) return true;
+    if (a.rows > kRowsPerLaunch) {
+        for (int64_t r = 0; r < a.rows; r += kRowsPerLaunch)
+            if (!launch_token_logprobs(rows_of(a, r, std::min(kRowsPerLaunch, a.rows - r), dtype_size(t)), t, st)) return false;
+        return true;
+    }
     return with_logit(t, [&](auto e) {
         using E = decltype(e);
         constexpr int W = 16 / sizeof(typename E::S);
@@ -390,6 +411,18 @@ bool launch_token_logprobs(const LogprobArgs &a, DType t, hipStream_t st) {
 
 bool launch_token_logprobs_grad(const LogprobGradArgs &g, DType t, hipStream_t st) {
     if (g.fwd.rows == 0) return true;
+    if (g.fwd.rows > kRowsPerLaunch) {
+        for (int64_t r = 0; r < g.fwd.rows; r += kRowsPerLaunch) {
+            LogprobGradArgs part = g;
+            part.fwd = rows_of(g.fwd, r, std::min(kRowsPerLaunch, g.fwd.rows - r), dtype_size(t));
+            if (g.g_logprob) part.g_logprob += r;
+            if (g.g_entropy) part.g_entropy += r;
+            if (g.g_top) part.g_top += r * g.fwd.top_k;
+            part.d_logits = static_cast<uint8_t *>(g.d_logits) + dtype_size(t) * g.fwd.vocab * r;
+            if (!launch_token_logprobs_grad(part, t, st)) return false;
+        }
+        return true;
+    }
     return with_logit(t, [&](auto e) {
         using E = decltype(e);
         constexpr int T = 256;

@@ -25,6 +25,7 @@ constexpr float kMuonScaleA = 1024.0f; // entries of A:  |a| <= 4^2   -> 16384
 constexpr float kMuonScaleP = 4096.0f; // entries of P:  |p| <= 12    -> 49152
 constexpr int kMuonPad = 64;           // X, A and P are padded to this with zeros, which the iteration keeps zero
 constexpr int kMuonMaxMats = 48;       // entries of one launch (they travel in the kernel arguments)
+constexpr int kMuonMaxSmall = 1 << 21; // matrices of one workgroup of 1024 in a launch, which has fewer than 2^32 threads
 constexpr int kMuonMaxPartials = 512;  // partial sums of squares of one matrix
 constexpr int kMuonPrepBlock = 4096;   // elements one workgroup of the first pass takes at least
 constexpr size_t kMuonWorkspaceBudget = size_t(4) << 30; // matrices are taken in groups of at most this (or one)
@@ -63,14 +64,14 @@ inline int muon_pad(int64_t v) { return static_cast<int>((v + kMuonPad - 1) / kM
 // Splits the entries into groups that run one after the other in the same workspace; returns the workspace's size.
 inline size_t muon_plan(const std::vector<MuonEntry> &entries, size_t esize_g, size_t esize_w,
                         std::vector<std::vector<MuonEntry>> *groups) {
-    size_t need = 0, used = 0;
+    size_t need = 0, used = 0, small = 0; // small: matrices of the group that fit in LDS
     std::vector<MuonEntry> group;
     const auto flush = [&] {
         if (group.empty()) return;
         need = std::max(need, used);
         if (groups) groups->push_back(group);
         group.clear();
-        used = 0;
+        used = small = 0;
     };
     for (MuonEntry e : entries) {
         if (e.count == 0 || e.rows == 0 || e.cols == 0) continue;
@@ -81,9 +82,9 @@ inline size_t muon_plan(const std::vector<MuonEntry> &entries, size_t esize_g, s
             std::min<size_t>(kMuonMaxPartials, (elems + kMuonPrepBlock - 1) / kMuonPrepBlock));
         int left = e.count;
         while (left > 0) {
-            size_t room = left;
+            size_t room = kMuonMaxSmall - small;
             if (bytes > 0) room = used < kMuonWorkspaceBudget ? (kMuonWorkspaceBudget - used) / bytes : 0;
-            if ((room == 0 && used > 0) || static_cast<int>(group.size()) == kMuonMaxMats) {
+            if ((room == 0 && (used > 0 || bytes == 0)) || static_cast<int>(group.size()) == kMuonMaxMats) {
                 flush();
                 continue;
             }
@@ -92,6 +93,7 @@ inline size_t muon_plan(const std::vector<MuonEntry> &entries, size_t esize_g, s
             part.off = used;
             group.push_back(part);
             used += bytes * part.count;
+            small += bytes == 0 ? part.count : 0;
             left -= part.count;
             e.g = static_cast<const uint8_t *>(e.g) + esize_g * elems * part.count;
             e.w = static_cast<uint8_t *>(e.w) + esize_w * elems * part.count;

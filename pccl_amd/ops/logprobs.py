@@ -6,6 +6,7 @@ the logits in their own type: no fp32 copy, no log-softmax tensor. GPU tensors r
 """
 from __future__ import annotations
 
+from operator import index
 from typing import NamedTuple, Optional
 
 import torch
@@ -178,6 +179,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top_k: int = 
     backward only queue kernels, so both may be captured into a graph. (Before a backward pass is captured, drop the
     results of eager calls on the same leaves: torch ends the process when their graph is still alive.)
     """
+    top_k, ignore_index = index(top_k), index(ignore_index)
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"token_logprobs: logits need a vocabulary dimension, got shape {tuple(logits.shape)}")
     if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
@@ -198,6 +200,6 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top_k: int = 
     elif logits.device.type != "cpu":
         raise ValueError(f"token_logprobs: no kernel for device {logits.device}")
     if logits.requires_grad and torch.is_grad_enabled():
-        return TokenLogprobs(*_TokenLogprobs.apply(logits, targets, int(top_k), int(ignore_index)))
-    logprob, entropy, _, top_lp, top_ix = _forward(logits, targets, int(top_k), int(ignore_index))
+        return TokenLogprobs(*_TokenLogprobs.apply(logits, targets, top_k, ignore_index))
+    logprob, entropy, _, top_lp, top_ix = _forward(logits, targets, top_k, ignore_index)
     return TokenLogprobs(logprob, entropy, top_lp, top_ix)

@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 import math
 from functools import lru_cache
+from operator import index
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -88,7 +89,7 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence[flo
     result one rounding more than bf16's own. A zero matrix gives zero, one with a NaN or an infinity gives NaN.
     Non-contiguous input is copied. ``out`` (contiguous, of x's shape and type) may be ``x`` itself.
     """
-    coefficients, steps = tuple(coefficients), int(steps)
+    coefficients, steps = tuple(coefficients), index(steps)
     _check_coefficients(coefficients, steps)
     if x.dim() < 2:
         raise ValueError(f"orthogonalize: a matrix or a stack of them, got shape {tuple(x.shape)}")
@@ -102,6 +103,8 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence[flo
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or not out.is_contiguous():
         raise ValueError("orthogonalize: out must be contiguous and match x in shape, type and device")
+    elif torch.is_grad_enabled() and out.requires_grad:
+        raise RuntimeError("orthogonalize: out requires a gradient: call it under no_grad")
     if x.numel() == 0:
         return out
     if x.device.type == "cpu":
@@ -152,9 +155,10 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
 
     ``params``: contiguous 2-D, one type of fp32 / bf16 / fp16; ``grads``: of their shapes, one type of the same three,
     non-contiguous ones are copied; ``momentum_buffers``: contiguous fp32. All on one device, none of them sharing
-    memory with another (a parameter listed twice is refused). Equal calls give equal bits on every peer.
+    memory with another (a parameter listed twice is refused; a gradient may serve several parameters). Equal calls give
+    equal bits on every peer. The call may be captured into a graph, which then keeps its learning rate.
     """
-    coefficients, steps = tuple(coefficients), int(steps)
+    coefficients, steps = tuple(coefficients), index(steps)
     check_muon("muon_step", lr, weight_decay, momentum, steps, coefficients, eps, adjust_lr)
     if not len(params) == len(grads) == len(momentum_buffers):
         raise ValueError(f"muon_step: {len(params)} parameters, {len(grads)} gradients and {len(momentum_buffers)} "
@@ -198,10 +202,12 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
         torch.autograd.graph.increment_version([t for e in work for t in (e[2], e[4])])
         return
     with torch.no_grad():
-        written = [t for e in work for t in (e[2], e[4])]
-        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in written)
-        if any(x[1] > y[0] for x, y in zip(spans, spans[1:])):
-            raise ValueError("muon_step: a tensor that is written shares memory with another one of the call")
+        end = written_end = 0  # furthest end so far, of any tensor / of the written ones
+        for start, stop, written in sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), k > 2)
+                                           for e in work for k, t in ((2, e[3]), (3, e[2]), (4, e[4]))):
+            if start < written_end or (written and start < end):
+                raise ValueError("muon_step: a tensor that is written shares memory with another one of the call")
+            end, written_end = max(end, stop), max(written_end, stop if written else 0)
         for (_, _, p, g, b), al in zip(work, alpha):
             g = g.float()
             b.add_(g - b, alpha=1.0 - momentum)

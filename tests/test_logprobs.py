@@ -298,6 +298,8 @@ def test_refusals(device):
             token_logprobs(x, t, top_k=bad)
     with pytest.raises(ValueError, match="top_k"):
         token_logprobs(x.repeat(1, 10), t, top_k=65)
+    with pytest.raises(TypeError, match="integer"):
+        token_logprobs(x, t, top_k=1.5)
     with pytest.raises(TypeError, match="int64"):
         token_logprobs(x, t.int())
     with pytest.raises(TypeError, match="fp32"):
@@ -373,3 +375,25 @@ def test_offsets_past_32_bits(hip):
     close(r.logprob[-3:], s.logprob.cpu(), 2 * sum_error(vocab))
     close(d[-3:], e.cpu(), e.cpu().double().abs() * 2.0 ** -7 + 1e-9)
     assert r.top_index[0].tolist() == [0, 1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("top_k", [0, 2])
+def test_more_rows_than_a_launch_has(hip, top_k):
+    """2^26 + 3 short rows: equal rows have equal results, wherever they stand."""
+    rows, vocab = (1 << 26) + 3, 5
+    few, few_t = make((7, vocab), torch.float16, hip)
+    x = few.repeat(rows // 7 + 1, 1)[:rows].requires_grad_()
+    t = few_t.repeat(rows // 7 + 1)[:rows]
+    r = token_logprobs(x, t, top_k=top_k)
+    results = [y for y in r if y is not None]
+    d, = torch.autograd.grad([y for y in results if y.requires_grad], x,
+                             [torch.ones_like(y) for y in results if y.requires_grad])
+    leaf = few.clone().requires_grad_()
+    s = [y for y in token_logprobs(leaf, few_t, top_k=top_k) if y is not None]
+    e, = torch.autograd.grad([y for y in s if y.requires_grad], leaf, [torch.ones_like(y) for y in s if y.requires_grad])
+    n = rows // 7
+    for got, want in zip(results + [d], s + [e]):
+        got, want = got.detach(), want.detach()
+        assert bool((got[:7 * n].view(n, 7, -1) == want.reshape(7, -1)).all())
+        assert torch.equal(got[7 * n:], want[:rows - 7 * n])

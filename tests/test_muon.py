@@ -187,6 +187,8 @@ def test_orthogonalize_refusals(device):
     for bad in (torch.empty(5, 6, device=device), x.half(), torch.empty(5, 6, device=device).T):
         with pytest.raises(ValueError, match="out"):
             orthogonalize(x, out=bad)
+    with pytest.raises(RuntimeError, match="no_grad"):
+        orthogonalize(x, out=torch.empty_like(x, requires_grad=True))
     for eps in (0.0, -1.0, math.nan, math.inf):
         with pytest.raises(ValueError, match="eps"):
             orthogonalize(x, eps=eps)
@@ -236,6 +238,16 @@ def test_more_matrices_than_a_group(hip):
     muon_step(params, grads, moms, lr=-1.0, weight_decay=0.0, momentum=0.0, adjust_lr="none")
     for p, g in zip(params, grads):
         assert torch.equal(p, orthogonalize(g))
+
+
+@pytest.mark.gpu
+def test_more_matrices_than_a_launch_has(hip):
+    """2^22 + 3 matrices of one workgroup each."""
+    x = gradient((7, 2, 3), 5, hip)
+    n = (1 << 22) + 3
+    got = orthogonalize(x.repeat(n // 7 + 1, 1, 1)[:n])
+    want = orthogonalize(x)
+    assert bool((got[:n // 7 * 7].view(-1, 7, 2, 3) == want).all()) and torch.equal(got[n // 7 * 7:], want[:n % 7])
 
 
 def model_step(p, g, b, lr, wd, mu, nesterov, factor, steps=5):
@@ -306,6 +318,10 @@ def test_muon_step_refusals(device):
         muon_step([p, p], [g, g], [b, b.clone()], **kw)
     with pytest.raises(ValueError, match="shares memory"):
         muon_step([p, p.clone()], [g, g], [b, b], **kw)
+    with pytest.raises(ValueError, match="shares memory"):
+        muon_step([p, p.clone()], [g, p], [b, b.clone()], **kw)
+    with pytest.raises(ValueError, match="shares memory"):
+        muon_step([p], [b], [b], **kw)
     big = torch.zeros(40, device=device)
     with pytest.raises(ValueError, match="shares memory"):
         muon_step([big[:30].view(6, 5), big[10:].view(6, 5)], [g, g], [b, b.clone()], **kw)

@@ -229,7 +229,7 @@ def fill_grads(params, turn):
 def test_state_dict(device, dtype, tmp_path):
     """A run that is saved and resumed goes on bit for bit; the momentum of bf16 matrices stays fp32."""
     def optimizer(params):
-        return Muon(params[:2], params[2:], lr=0.02, weight_decay=0.1)
+        return Muon(params[:2], params[2:], lr=0.02, weight_decay=0.1, fused=device.type == "cuda")
     params = small_params(device, dtype)
     opt = optimizer(params)
     for turn in range(2):
