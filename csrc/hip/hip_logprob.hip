@@ -3,8 +3,10 @@
 //
 // Memory bound: the forward reads every logit once, the backward reads and writes each once. One workgroup per row
 // holds a running (max, sum of exponentials, sum of exponentials times distance) per thread in fp32 and joins them at
-// the end, so the row is never stored in a wider type. The sums' order is fixed by (row length, workgroup size), so
-// equal calls give equal bits.
+// the end, so the row is never stored in a wider type. The sums' order is fixed by row length and workgroup size, so
+// equal calls give equal bits. 12288 x 50304 bf16: forward 210 us, 5.9 TB/s (with 20 alternatives 239 us); backward
+// 466 us, 5.3 TB/s; a large copy moves 4.8 TB/s. One row of 50304 takes 7 us, 10 with alternatives, where a call's
+// host side takes 13 to 17: a row is not split over workgroups.
 //
 // Top alternatives need no second pass over the row: each thread also knows its best value and the block of the row
 // where it first stood, and 64 groups of threads the best of these. Ordered by (value, earlier block), the k-th best of
@@ -380,7 +382,8 @@ bool launch_token_logprobs(const LogprobArgs &a, DType t, hipStream_t st) {
     if (a.rows == 0) return true;
     if (a.rows > kRowsPerLaunch) {
         for (int64_t r = 0; r < a.rows; r += kRowsPerLaunch)
-            if (!launch_token_logprobs(rows_of(a, r, std::min(kRowsPerLaunch, a.rows - r), dtype_size(t)), t, st)) return false;
+            if (!launch_token_logprobs(rows_of(a, r, std::min(kRowsPerLaunch, a.rows - r), dtype_size(t)), t, st))
+                return false;
         return true;
     }
     return with_logit(t, [&](auto e) {

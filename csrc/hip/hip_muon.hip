@@ -250,7 +250,8 @@ __global__ __launch_bounds__(256) void k_muon_start(MuonTable t, MuonParams p) {
         for (int j = 0; j < 8; ++j) v[j] = tile[r][x + j];
         half8 hi, lo;
         split_fp16<8>(v, hi, lo);
-        *reinterpret_cast<half8 *>(q.x0 + panel_at<PAIRS>(e.mp, m0 + r, n0 + x) + (low ? PAIRS ? 16 : q.xs : 0)) = low ? lo : hi;
+        _Float16 *to = q.x0 + panel_at<PAIRS>(e.mp, m0 + r, n0 + x) + (low ? PAIRS ? 16 : q.xs : 0);
+        *reinterpret_cast<half8 *>(to) = low ? lo : hi;
     }
 }
 
@@ -335,9 +336,14 @@ __device__ __forceinline__ int place_of_block() {
 // the N side's of kGram and kPoly, which multiply by a transpose; kApply's and kFinal's N side is X itself, whose
 // fragments are transposed on their way out of LDS. Both sides travel straight to LDS, a panel of the sum at a time.
 // SPLIT: three products of the parts. PAIRS: X and P lie in pairs. The MFMA's first operand is the N side: a lane then
-// holds 4 neighbouring columns of one row.
-// WV waves share a tile, two along m. KG groups of them take the panels in turn and add their sums up at the end: with few tiles this fills the CUs.
-// Of ST panels in a group's part of LDS one is multiplied, the others are on their way.
+// holds 4 neighbouring columns of one row. WV waves share a tile, two along m. KG groups of them take the panels in turn
+// and add their sums up at the end: with few tiles this fills the CUs. Of ST panels in a group's part of LDS one is
+// multiplied, the others are on their way.
+//
+// What bounds it, 2 x 4096 x 4096: the matrix cores under the card's power limit. P X with three products runs at 1230
+// TFLOP/s issued (670 us), where the library's fp16 product of 8192^3 reaches 1170; with one product 905
+// (304 us). 12 x 768 x 768, 10 to 15 GFLOP a stage: 19 to 30 us, of which 9 do not depend on the length of the sum, the
+// start of a launch and the results on their way to memory behind it (14 to 28 MB: without the stores 12 to 25 us).
 template<int KIND, int BM, int BN, int WV, int KG, int ST, bool SPLIT, bool PAIRS, DType W>
 __global__ __launch_bounds__(64 * WV * KG, KG == 1 ? 2 : 4) void k_muon_product(MuonTable t, MuonStage st) {
     constexpr int WM = BM / 2, WN = BN / (WV / 2), MT = WM / 32, NT = WN / 32;
@@ -394,7 +400,9 @@ __global__ __launch_bounds__(64 * WV * KG, KG == 1 ? 2 : 4) void k_muon_product(
         if constexpr (NN) { // BK rows of BN / BK panels
             const int j = wave * NI + k, panels = e.np / BK;
             const int pn = n0 / BK + j / (BK / 16);
-            np[k] = ns + (static_cast<size_t>(pn < panels ? pn : panels - 1) * rows + group * BK + j % (BK / 16) * 16 + lrow) * 32 +
+            np[k] = ns +
+                    (static_cast<size_t>(pn < panels ? pn : panels - 1) * rows + group * BK + j % (BK / 16) * 16 + lrow) *
+                        32 +
                     (lpiece ^ (SPLIT ? (j & 1) << 1 : 0)) * 8;
         } else {
             const int r = n0 + (wave * NI + k) * 16 + lrow;
@@ -688,7 +696,9 @@ __global__ __launch_bounds__(64 * WV * KG, KG == 1 ? 2 : 4) void k_muon_product(
 // Everything for a matrix that fits in LDS, by one workgroup of 16 waves: X, and A / P in one place, in paired panels
 // as above and with three products throughout. The stages above would take 17 launches of a few busy CUs. Every wave
 // has one 32 x 32 tile of A or of A A; where there are only four (MP = 64), four waves each sum over a quarter of the
-// panels and then finish a quarter of the tile.
+// panels and then finish a quarter of the tile. Bound by the chain of LDS reads, products and barriers of the few
+// waves: 64 x 64 about 3 us a step (21 us the call), 64 x 256 4.3, 128 x 128 7; as 17 launches of the stages the call
+// of 64 x 64 took 77 us.
 template<int MP, int NP, DType G, DType W>
 __global__ __launch_bounds__(1024) void k_muon_small(MuonTable t, MuonParams p) {
     using S = typename Elem<G>::S;

@@ -25,7 +25,7 @@ constexpr float kMuonScaleA = 1024.0f; // entries of A:  |a| <= 4^2   -> 16384
 constexpr float kMuonScaleP = 4096.0f; // entries of P:  |p| <= 12    -> 49152
 constexpr int kMuonPad = 64;           // X, A and P are padded to this with zeros, which the iteration keeps zero
 constexpr int kMuonMaxMats = 48;       // entries of one launch (they travel in the kernel arguments)
-constexpr int kMuonMaxSmall = 1 << 21; // matrices of one workgroup of 1024 in a launch, which has fewer than 2^32 threads
+constexpr int kMuonMaxSmall = 1 << 21;  // matrices of one workgroup in a launch, which has fewer than 2^32 threads
 constexpr int kMuonMaxPartials = 512;  // partial sums of squares of one matrix
 constexpr int kMuonPrepBlock = 4096;   // elements one workgroup of the first pass takes at least
 constexpr size_t kMuonWorkspaceBudget = size_t(4) << 30; // matrices are taken in groups of at most this (or one)
@@ -77,7 +77,8 @@ inline size_t muon_plan(const std::vector<MuonEntry> &entries, size_t esize_g, s
         if (e.count == 0 || e.rows == 0 || e.cols == 0) continue;
         e.mp = muon_pad(std::min(e.rows, e.cols));
         e.np = muon_pad(std::max(e.rows, e.cols));
-        const size_t elems = static_cast<size_t>(e.rows) * e.cols, bytes = muon_fits_lds(e.mp, e.np) ? 0 : muon_matrix_bytes(e.mp, e.np);
+        const size_t elems = static_cast<size_t>(e.rows) * e.cols;
+        const size_t bytes = muon_fits_lds(e.mp, e.np) ? 0 : muon_matrix_bytes(e.mp, e.np);
         e.partials = static_cast<int>(
             std::min<size_t>(kMuonMaxPartials, (elems + kMuonPrepBlock - 1) / kMuonPrepBlock));
         int left = e.count;

@@ -52,8 +52,8 @@ class Muon(torch.optim.Optimizer):
         group = self.param_groups[-1]
         try:
             if group["muon"]:
-                check_muon("Muon", *(group[k] for k in ("lr", "weight_decay", "momentum", "steps", "coefficients", "eps",
-                                                       "adjust_lr")))
+                check_muon("Muon", *(group[k] for k in ("lr", "weight_decay", "momentum", "steps", "coefficients",
+                                                        "eps", "adjust_lr")))
                 for p in group["params"]:
                     if hasattr(p, "placements"):  # not isinstance: importing DTensor takes half a second
                         raise TypeError("Muon: a sharded parameter (DTensor); matrices must be whole")

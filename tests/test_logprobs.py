@@ -391,7 +391,8 @@ def test_more_rows_than_a_launch_has(hip, top_k):
                              [torch.ones_like(y) for y in results if y.requires_grad])
     leaf = few.clone().requires_grad_()
     s = [y for y in token_logprobs(leaf, few_t, top_k=top_k) if y is not None]
-    e, = torch.autograd.grad([y for y in s if y.requires_grad], leaf, [torch.ones_like(y) for y in s if y.requires_grad])
+    e, = torch.autograd.grad([y for y in s if y.requires_grad], leaf,
+                             [torch.ones_like(y) for y in s if y.requires_grad])
     n = rows // 7
     for got, want in zip(results + [d], s + [e]):
         got, want = got.detach(), want.detach()

@@ -125,7 +125,8 @@ def check_step(matrices, others, before, grads, twin, adamw, lr, wd):
     for p, (p0, b0), g in zip(matrices, before, grads):
         factor = 0.2 * math.sqrt(max(p.shape))
         want, _, u = model_step(p0, g, b0, lr, wd, 0.95, True, factor)
-        tol = 3 * deviation(u, False) * 4 * lr * factor + want.abs() * U * 1.01 + 4 * U * (p0.double().abs() + lr * factor)
+        tol = 3 * deviation(u, False) * 4 * lr * factor + want.abs() * U * 1.01
+        tol = tol + 4 * U * (p0.double().abs() + lr * factor)
         assert bool(((p.detach().double() - want).abs() <= tol).all())
     for p, q in zip(others, twin):
         q.grad = p.grad.clone()
