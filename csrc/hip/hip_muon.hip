@@ -693,26 +693,25 @@ __global__ __launch_bounds__(64 * WV * KG, KG == 1 ? 2 : 4) void k_muon_product(
     }
 }
 
-// Everything for a matrix that fits in LDS, by one workgroup of 16 waves: X, and A / P in one place, in paired panels
-// as above and with three products throughout. The stages above would take 17 launches of a few busy CUs. Every wave
-// has one 32 x 32 tile of A or of A A; where there are only four (MP = 64), four waves each sum over a quarter of the
-// panels and then finish a quarter of the tile. Bound by the chain of LDS reads, products and barriers of the few
-// waves: 64 x 64 about 3 us a step (21 us the call), 64 x 256 4.3, 128 x 128 7; as 17 launches of the stages the call
-// of 64 x 64 took 77 us.
-template<int MP, int NP, DType G, DType W>
-__global__ __launch_bounds__(1024) void k_muon_small(MuonTable t, MuonParams p) {
+// Everything for a matrix that fits in LDS, by one workgroup: X, and A / P in one place, in paired panels as above and
+// with three products throughout. A wave has whole 32 x 32 tiles of the products, so nothing is joined between waves,
+// and keeps its own entries of X and A in registers from product to product. Bound by LDS reads, products and barriers
+// in turn; us of a call of orthogonalize / the Muon step: 64 x 64 13 / 15 (4 waves; sharing each tile's sum between 2
+// or 4 waves 17 / 21), 64 x 256 26 / 29 (8 waves; 4, which read least, 36), 256 x 64 27 / 31, 128 x 128 38 / 41 (16
+// waves; 8 40 / 43). 1000 of 64 x 64 35 us. The 17 launches of the stages took 77 for 64 x 64.
+template<int MP, int NP, int NW, DType G, DType W>
+__global__ __launch_bounds__(64 * NW) void k_muon_small(MuonTable t, MuonParams p) {
     using S = typename Elem<G>::S;
     using WS = typename Elem<W>::S;
     constexpr int MB = MP / 32;
-    constexpr int KS = 16 / (MB * MB);              // waves that share a tile of A
-    constexpr int GB = 4 / KS;                      // groups of 4 columns that a wave finishes of it
-    constexpr int AW = (MB * (NP / 32) + 15) / 16;  // tiles of X per wave
-    constexpr int E = MP * NP / 8192 > 0 ? MP * NP / 8192 : 1; // groups of 8 elements per thread
-    static_assert(MP == 64 || MP == 128);
+    constexpr int NA = NW < MB * MB ? NW : MB * MB; // waves that have tiles of A
+    constexpr int RA = MB * MB / NA;                // tiles of A of such a wave, one under the other
+    constexpr int RM = MB * (NP / 32) / NW;         // tiles of X of a wave, one under the other
+    constexpr int E = MP * NP / (512 * NW);         // groups of 8 elements per thread
+    static_assert((MP == 64 || MP == 128) && RA * NA == MB * MB && RM * NW == MB * (NP / 32) && MB % RM == 0);
     __shared__ __attribute__((aligned(16))) uint8_t lx[MP * NP * 4];
     __shared__ __attribute__((aligned(16))) uint8_t la[MP * MP * 4];
-    __shared__ float4 part[KS > 1 ? MB * MB * KS * (KS - 1) * 64 : 1];
-    __shared__ double sums[16];
+    __shared__ double sums[NW];
 
     const int i = entry_of(t, blockIdx.x);
     const MuonEntry &e = t.e[i];
@@ -733,17 +732,21 @@ __global__ __launch_bounds__(1024) void k_muon_small(MuonTable t, MuonParams p) 
     // of a wave lie along the caller's rows: 8 x 8 groups, or 64 rows where X is the transpose.
     float u[E][8];
     int gm[E], gn[E];
-    bool whole[E];
+    bool whole[E], tall[E];
 #pragma unroll
     for (int k = 0; k < E; ++k) {
-        const int unit = threadIdx.x + 1024 * k, in = unit & 63, blk = unit >> 6;
+        const int unit = threadIdx.x + 64 * NW * k, in = unit & 63, blk = unit >> 6;
         gm[k] = flip ? blk % (MP / 64) * 64 + in : blk % (MP / 8) * 8 + (in >> 3);
         gn[k] = flip ? blk / (MP / 64) * 8 : (blk / (MP / 8) * 8 + (in & 7)) * 8;
         whole[k] = !flip && gm[k] < ms && gn[k] + 8 <= ns; // 8 neighbours in the caller's memory too
+        tall[k] = flip && gm[k] < ms && gn[k] + 8 <= ns;   // 8 loads or stores without a condition each
         if (whole[k]) {
             const Run<S, 8> v = *reinterpret_cast<const Run<S, 8> *>(g + place(gm[k], gn[k]));
 #pragma unroll
             for (int j = 0; j < 8; ++j) u[k][j] = static_cast<float>(v.v[j]);
+        } else if (tall[k]) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) u[k][j] = static_cast<float>(g[place(gm[k], gn[k] + j)]);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -756,6 +759,9 @@ __global__ __launch_bounds__(1024) void k_muon_small(MuonTable t, MuonParams p) 
         for (int k = 0; k < E; ++k) {
             if (whole[k]) {
                 old[k] = *reinterpret_cast<const Run<float, 8> *>(mom + place(gm[k], gn[k]));
+            } else if (tall[k]) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) old[k].v[j] = mom[place(gm[k], gn[k] + j)];
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
@@ -772,6 +778,9 @@ __global__ __launch_bounds__(1024) void k_muon_small(MuonTable t, MuonParams p) 
             }
             if (whole[k]) {
                 *reinterpret_cast<Run<float, 8> *>(mom + place(gm[k], gn[k])) = old[k];
+            } else if (tall[k]) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) mom[place(gm[k], gn[k] + j)] = old[k].v[j];
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
@@ -790,7 +799,7 @@ __global__ __launch_bounds__(1024) void k_muon_small(MuonTable t, MuonParams p) 
     __syncthreads();
     sum = 0.0;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) sum += sums[k];
+    for (int k = 0; k < NW; ++k) sum += sums[k];
     const double norm = sqrt(sum);
     const double scale = static_cast<double>(kMuonScaleX) / (norm > p.eps || norm != norm ? norm : p.eps);
 #pragma unroll
@@ -854,129 +863,134 @@ __global__ __launch_bounds__(1024) void k_muon_small(MuonTable t, MuonParams p) 
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] = join_fp16(h[r], l[r]);
     };
-    // this wave's tile of `base` times its own transpose, complete in the groups GB * q ..
-    const int gt = wave % (MB * MB), gr = gt % MB * 32, gc = gt / MB * 32, gq = wave / (MB * MB);
-    const auto square = [&](const uint8_t *base, int panels, float (&out)[GB][4]) {
-        float16v acc = {};
-        for (int s = gq; s < panels; s += KS) {
-            const half8 m[2] = {frag(base, gr, s, 0), frag(base, gr, s, 1)};
-            const half8 n[2] = {frag(base, gc, s, 0), frag(base, gc, s, 1)};
-            acc = mul3(acc, n, m);
-        }
-        if constexpr (KS == 1) {
-            __syncthreads();
+    // where this wave's tiles lie: of A in rows ar + 32 k, of X in rows xr + 32 k
+    const int ar = wave * RA % MB * 32, ac = wave * RA / MB * 32;
+    const int xr = wave * RM % MB * 32, xc = wave * RM / MB * 32;
+    const bool has_a = NA == NW || wave < NA, has_x = NP == MP || xc < np;
+    // this wave's tiles of `base` times its own transpose
+    const auto square = [&](const uint8_t *base, int panels, float16v (&out)[RA]) {
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
+        for (int k = 0; k < RA; ++k) out[k] = float16v{};
+#pragma unroll (MP == 128 ? 2 : 4)
+        for (int s = 0; s < panels; ++s) {
+            const half8 n[2] = {frag(base, ac, s, 0), frag(base, ac, s, 1)};
 #pragma unroll
-                for (int r = 0; r < 4; ++r) out[b][r] = acc[4 * b + r];
-        } else {
-            static_assert(KS == 4 && GB == 1);
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                if (b == gq) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) out[0][r] = acc[4 * b + r];
-                } else { // to the wave that finishes group b
-                    part[((gt * 4 + b) * 3 + (gq - b + 3) % 4) * 64 + lane] =
-                        make_float4(acc[4 * b], acc[4 * b + 1], acc[4 * b + 2], acc[4 * b + 3]);
-                }
-            }
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < 3; ++k) {
-                const float4 o = part[((gt * 4 + gq) * 3 + k) * 64 + lane];
-                out[0][0] += o.x;
-                out[0][1] += o.y;
-                out[0][2] += o.z;
-                out[0][3] += o.w;
+            for (int k = 0; k < RA; ++k) {
+                const half8 m[2] = {frag(base, ar + 32 * k, s, 0), frag(base, ar + 32 * k, s, 1)};
+                out[k] = mul3(out[k], n, m);
             }
         }
     };
-    const int tiles = MB * (np / 32);
 
-    for (int step = 0; step < p.steps; ++step) {
-        __syncthreads(); // X is written
-        float sq[GB][4];
-        square(lx, np / 16, sq);
+    __syncthreads(); // X is written
+    float x[RM][16]; // this wave's entries of X
+    if (has_x)
 #pragma unroll
-        for (int k = 0; k < GB; ++k) {
-            const int b = GB * gq + k;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) sq[k][r] *= kMuonScaleA / (kMuonScaleX * kMuonScaleX);
-            put4(la, group_at(gr, gc, b), b, sq[k]);
-        }
-        __syncthreads(); // A is written
-        square(la, MP / 16, sq); // ends behind a barrier: A's products are read
-#pragma unroll
-        for (int k = 0; k < GB; ++k) {
-            const int b = GB * gq + k;
-            float v[4];
-            get4(la, group_at(gr, gc, b), b, v); // A until here, P from now on: the same lane's
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                v[r] = __builtin_fmaf(p.b * (kMuonScaleP / kMuonScaleA), v[r],
-                                      sq[k][r] * (p.c * (kMuonScaleP / (kMuonScaleA * kMuonScaleA))));
-            put4(la, group_at(gr, gc, b), b, v);
-        }
-        __syncthreads(); // P is written
-        const bool last = step == p.steps - 1;
-        float16v xa[AW];
-        Run<WS, 4> old[AW][4];
-#pragma unroll
-        for (int k = 0; k < AW; ++k) {
-            const int tile = wave + 16 * k, mt = tile % MB * 32, nt = tile / MB * 32;
-            if (tile >= tiles) break;
-            if (last && mom) {
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const int m = mt + l32, n = nt + 4 * half + 8 * b;
-                    if (!flip && m < ms && n + 4 <= ns) {
-                        old[k][b] = *reinterpret_cast<const Run<WS, 4> *>(w + place(m, n));
-                    } else {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) old[k][b].v[r] = m < ms && n + r < ns ? w[place(m, n + r)] : WS{};
-                    }
-                }
-            }
-            xa[k] = float16v{};
-#pragma unroll 2
-            for (int s = 0; s < MP / 16; ++s) {
-                const half8 m[2] = {frag(la, mt, s, 0), frag(la, mt, s, 1)};
-                const half8 n[2] = {frag_t(lx, 16 * s, nt, 0), frag_t(lx, 16 * s, nt, 1)};
-                xa[k] = mul3(xa[k], n, m);
-            }
-        }
-        __syncthreads(); // X is read
-#pragma unroll
-        for (int k = 0; k < AW; ++k) {
-            const int tile = wave + 16 * k, mt = tile % MB * 32, nt = tile / MB * 32;
-            if (tile >= tiles) break;
+        for (int k = 0; k < RM; ++k)
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
                 float v[4];
-                get4(lx, group_at(mt, nt, b), b, v);
+                get4(lx, group_at(xr + 32 * k, xc, b), b, v);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = __builtin_fmaf(p.a, v[r], xa[k][4 * b + r] * (1.0f / kMuonScaleP));
-                if (!last) {
-                    put4(lx, group_at(mt, nt, b), b, v);
-                    continue;
-                }
-                const int m = mt + l32, n = nt + 4 * half + 8 * b;
-                Run<WS, 4> now;
+                for (int r = 0; r < 4; ++r) x[k][4 * b + r] = v[r];
+            }
+    for (int step = 0; step < p.steps; ++step) {
+        float16v sq[RA], aa[RA];
+        if (has_a) {
+            square(lx, NP == MP ? MP / 16 : np / 16, sq);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float o = v[r] * (1.0f / kMuonScaleX);
-                    now.v[r] = static_cast<WS>(mom ? static_cast<float>(old[k][b].v[r]) * p.decay - e.alpha * o : o);
+            for (int k = 0; k < RA; ++k)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    float v[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) v[r] = sq[k][4 * b + r] *= kMuonScaleA / (kMuonScaleX * kMuonScaleX);
+                    put4(la, group_at(ar + 32 * k, ac, b), b, v);
                 }
-                if (!flip && m < ms && n + 4 <= ns) {
-                    *reinterpret_cast<Run<WS, 4> *>(w + place(m, n)) = now;
-                } else {
+        }
+        __syncthreads(); // A is written
+        if (has_a) square(la, MP / 16, aa);
+        __syncthreads(); // A is read; P takes its place
+        if (has_a)
+#pragma unroll
+            for (int k = 0; k < RA; ++k)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    float v[4];
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        if (m < ms && n + r < ns) w[place(m, n + r)] = now.v[r];
+                        v[r] = __builtin_fmaf(p.b * (kMuonScaleP / kMuonScaleA), sq[k][4 * b + r],
+                                              aa[k][4 * b + r] * (p.c * (kMuonScaleP / (kMuonScaleA * kMuonScaleA))));
+                    put4(la, group_at(ar + 32 * k, ac, b), b, v);
+                }
+        __syncthreads(); // P is written
+        const bool last = step == p.steps - 1;
+        Run<WS, 4> old[RM][4];
+        float16v px[RM] = {};
+        if (has_x) {
+            if (last && mom) { // on their way while P X is computed
+#pragma unroll
+                for (int k = 0; k < RM; ++k)
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        const int m = xr + 32 * k + l32, n = xc + 4 * half + 8 * b;
+                        if (!flip && m < ms && n + 4 <= ns) {
+                            old[k][b] = *reinterpret_cast<const Run<WS, 4> *>(w + place(m, n));
+                        } else if (m < ms && n + 4 <= ns) {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) old[k][b].v[r] = w[place(m, n + r)];
+                        } else {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                old[k][b].v[r] = m < ms && n + r < ns ? w[place(m, n + r)] : WS{};
+                        }
+                    }
+            }
+#pragma unroll
+            for (int s = 0; s < MP / 16; ++s) {
+                const half8 n[2] = {frag_t(lx, 16 * s, xc, 0), frag_t(lx, 16 * s, xc, 1)};
+#pragma unroll
+                for (int k = 0; k < RM; ++k) {
+                    const half8 m[2] = {frag(la, xr + 32 * k, s, 0), frag(la, xr + 32 * k, s, 1)};
+                    px[k] = mul3(px[k], n, m);
                 }
             }
         }
+        __syncthreads(); // X is read
+        if (has_x)
+#pragma unroll
+            for (int k = 0; k < RM; ++k)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    float v[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        v[r] = x[k][4 * b + r] =
+                            __builtin_fmaf(p.a, x[k][4 * b + r], px[k][4 * b + r] * (1.0f / kMuonScaleP));
+                    if (!last) {
+                        put4(lx, group_at(xr + 32 * k, xc, b), b, v);
+                        continue;
+                    }
+                    const int m = xr + 32 * k + l32, n = xc + 4 * half + 8 * b;
+                    Run<WS, 4> now;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float o = v[r] * (1.0f / kMuonScaleX);
+                        now.v[r] =
+                            static_cast<WS>(mom ? static_cast<float>(old[k][b].v[r]) * p.decay - e.alpha * o : o);
+                    }
+                    if (!flip && m < ms && n + 4 <= ns) {
+                        *reinterpret_cast<Run<WS, 4> *>(w + place(m, n)) = now;
+                    } else if (m < ms && n + 4 <= ns) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) w[place(m, n + r)] = now.v[r];
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (m < ms && n + r < ns) w[place(m, n + r)] = now.v[r];
+                    }
+                }
+        if (!last) __syncthreads(); // X is written
     }
 }
 
@@ -1005,8 +1019,8 @@ template<int KIND, int BM, int BN, int WV, int KG, int ST, bool SPLIT, bool PAIR
 bool launch_product(MuonTable &t, const MuonStage &st, hipStream_t s) {
     const int64_t n = layout(t, [](const MuonEntry &e) { return product_tiles<BM, BN>(KIND, e); });
     if (n > INT32_MAX) return false;
-    return launch_ok(
-        [&] { k_muon_product<KIND, BM, BN, WV, KG, ST, SPLIT, PAIRS, W><<<dim3(static_cast<unsigned>(n)), 64 * WV * KG, 0, s>>>(t, st); });
+    const dim3 grid(static_cast<unsigned>(n));
+    return launch_ok([&] { k_muon_product<KIND, BM, BN, WV, KG, ST, SPLIT, PAIRS, W><<<grid, 64 * WV * KG, 0, s>>>(t, st); });
 }
 
 template<int KIND, bool SPLIT, bool PAIRS, DType W = DType::F32>
@@ -1042,18 +1056,18 @@ bool launch_stage(MuonTable &t, const MuonStage &st, hipStream_t s) {
 
 } // namespace
 
-template<int MP, int NP, DType G>
+template<int MP, int NP, int NW, DType G>
 static bool launch_small(MuonTable &t, DType wt, const MuonParams &p, hipStream_t s) {
     const int64_t n = layout(t, [](const MuonEntry &) { return 1; });
     if (n > INT32_MAX) return false;
     const dim3 grid(static_cast<unsigned>(n));
     return launch_ok([&] {
         if (wt == DType::F32)
-            k_muon_small<MP, NP, G, DType::F32><<<grid, 1024, 0, s>>>(t, p);
+            k_muon_small<MP, NP, NW, G, DType::F32><<<grid, 64 * NW, 0, s>>>(t, p);
         else if (wt == DType::BF16)
-            k_muon_small<MP, NP, G, DType::BF16><<<grid, 1024, 0, s>>>(t, p);
+            k_muon_small<MP, NP, NW, G, DType::BF16><<<grid, 64 * NW, 0, s>>>(t, p);
         else
-            k_muon_small<MP, NP, G, DType::F16><<<grid, 1024, 0, s>>>(t, p);
+            k_muon_small<MP, NP, NW, G, DType::F16><<<grid, 64 * NW, 0, s>>>(t, p);
     });
 }
 
@@ -1083,8 +1097,9 @@ bool launch_muon(const MuonEntry *entries, int n, DType gt, DType wt, const Muon
     };
     const bool started = with_grad([&](auto g) {
         constexpr DType G = decltype(g)::value;
-        if (square.n && !launch_small<128, 128, G>(square, wt, p, s)) return false;
-        if (narrow.n && !(np > 64 ? launch_small<64, 256, G>(narrow, wt, p, s) : launch_small<64, 64, G>(narrow, wt, p, s)))
+        if (square.n && !launch_small<128, 128, 16, G>(square, wt, p, s)) return false;
+        if (narrow.n && !(np > 64 ? launch_small<64, 256, 8, G>(narrow, wt, p, s)
+                                  : launch_small<64, 64, 4, G>(narrow, wt, p, s)))
             return false;
         if (t.n == 0) return true;
         int64_t blocks = layout(t, [](const MuonEntry &e) { return e.partials; });
