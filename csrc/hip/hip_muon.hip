@@ -1025,32 +1025,45 @@ bool launch_product(MuonTable &t, const MuonStage &st, hipStream_t s) {
 
 template<int KIND, bool SPLIT, bool PAIRS, DType W = DType::F32>
 bool launch_stage(MuonTable &t, const MuonStage &st, hipStream_t s) {
-    // Tiles by an estimate of a launch's time per panel of the sum, in us, fitted to what each took with n tiles per CU
-    // (n between the average and the fullest CU's, or that of the fullest where only one fits). In us, fp32, X X^T / P X,
-    // for 256 x 128, 128 x 128, 128 x 64, 64 x 64 by two groups of waves and by four:
-    //   1 x 1024 x 1024     45 / 48     29 / 32     22 / 24     14 / 16     13 / 15
-    //   12 x 768 x 768      42 / 48     31 / 41     29 / 45     30 / 54     40 / 70
-    //   4 x 1024 x 4096    157 / 102   103 / 106    93 / 114    89 / 157    99 / 188
-    //   2 x 4096 x 4096    491 / 670   435 / 724   471 / 830   603 / 1022  649 / 1137
-    const auto cost = [&](auto tiles_of, double per_tile, double fixed, bool one_fits = false) {
+    // Tiles by an estimate of a launch's time: some us, and for each panel of the sum the time of a tile times the tiles
+    // of a CU, between the average and the fullest CU's (where two fit a CU an odd one out takes a quarter longer, where
+    // one fits the fullest counts). Fitted to 44 calls in two types; the tiles chosen cost 1 % over the best of each launch
+    // on average. In us, fp32, X X^T / P X, for 256 x 128, 128 x 128, 128 x 64, 64 x 64 by two groups of waves and by
+    // four, 64 x 32 by four:
+    //   1 x 512 x 512       27 / 29     17 / 19     13 / 14      9 / 10      9 / 9       7 / 7
+    //   1 x 1024 x 1024     44 / 47     29 / 31     21 / 23     14 / 16     13 / 14     13 / 14
+    //   12 x 768 x 768      41 / 46     30 / 40     29 / 46     30 / 54     39 / 70     38 / 64
+    //   4 x 1024 x 4096    157 / 102   105 / 107    94 / 116    88 / 155   100 / 190   101 / 188
+    //   2 x 4096 x 4096    493 / 680   438 / 740   473 / 846   609 / 1023  658 / 1172  669 / 1254
+    double panels = 0.0, all = 0.0;
+    for (int i = 0; i < t.n; ++i) {
+        const double tiles = static_cast<double>(t.e[i].count) * product_tiles<64, 64>(KIND, t.e[i]);
+        panels += tiles * (KIND == kGram ? t.e[i].np : t.e[i].mp) / (SPLIT ? 16 : 32);
+        all += tiles;
+    }
+    panels /= all;
+    const auto cost = [&](auto tiles_of, double launch, double tile, bool two_fit = true) {
         int64_t tiles = 0;
         for (int i = 0; i < t.n; ++i) tiles += t.e[i].count * tiles_of(t.e[i]);
-        const double average = tiles / 256.0, fullest = static_cast<double>((tiles + 255) / 256);
-        return fixed + per_tile * (one_fits ? fullest : average <= 1.0 ? 1.0 : 0.5 * (average + fullest));
+        const int64_t fullest = (tiles + 255) / 256;
+        const double average = std::max(tiles / 256.0, 1.0);
+        return launch + panels * tile * (two_fit ? 0.5 * (average + fullest) + (fullest & 1) * 0.26 : fullest);
     };
-    const double est[5] = {
-        cost([](const MuonEntry &e) { return product_tiles<256, 128>(KIND, e); }, 0.62, 0.21),
-        cost([](const MuonEntry &e) { return product_tiles<128, 128>(KIND, e); }, 0.33, 0.16),
-        cost([](const MuonEntry &e) { return product_tiles<128, 64>(KIND, e); }, 0.22, 0.10),
-        cost([](const MuonEntry &e) { return product_tiles<64, 64>(KIND, e); }, 0.122, 0.12),
-        cost([](const MuonEntry &e) { return product_tiles<64, 64>(KIND, e); }, 0.20, 0.00, true),
+    const double est[6] = {
+        cost([](const MuonEntry &e) { return product_tiles<256, 128>(KIND, e); }, 6.0, 0.600),
+        cost([](const MuonEntry &e) { return product_tiles<128, 128>(KIND, e); }, 6.9, 0.313),
+        cost([](const MuonEntry &e) { return product_tiles<128, 64>(KIND, e); }, 4.5, 0.207),
+        cost([](const MuonEntry &e) { return product_tiles<64, 64>(KIND, e); }, 4.2, 0.125),
+        cost([](const MuonEntry &e) { return product_tiles<64, 64>(KIND, e); }, 4.4, 0.149, false),
+        cost([](const MuonEntry &e) { return product_tiles<64, 32>(KIND, e); }, 4.2, 0.084),
     };
-    switch (std::min_element(est, est + 5) - est) {
+    switch (std::min_element(est, est + 6) - est) {
         case 0: return launch_product<KIND, 256, 128, 4, 1, 3, SPLIT, PAIRS, W>(t, st, s);
         case 1: return launch_product<KIND, 128, 128, 4, 1, 3, SPLIT, PAIRS, W>(t, st, s);
         case 2: return launch_product<KIND, 128, 64, 4, 1, 3, SPLIT, PAIRS, W>(t, st, s);
         case 3: return launch_product<KIND, 64, 64, 4, 2, 3, SPLIT, PAIRS, W>(t, st, s);
-        default: return launch_product<KIND, 64, 64, 4, 4, 3, SPLIT, PAIRS, W>(t, st, s);
+        case 4: return launch_product<KIND, 64, 64, 4, 4, 3, SPLIT, PAIRS, W>(t, st, s);
+        default: return launch_product<KIND, 64, 32, 2, 4, 3, SPLIT, PAIRS, W>(t, st, s);
     }
 }
 
