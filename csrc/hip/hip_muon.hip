@@ -1096,7 +1096,7 @@ bool launch_muon(const MuonEntry *entries, int n, DType gt, DType wt, const Muon
     // Three products everywhere: where the result has more bits than one product, and for small matrices, whose sums are
     // too short to average the roundings of one product out (sides below 200: up to 1.46 times the error of the bf16
     // result's own rounding, against 1.00; 1.1 to 1.36 from 320 to 2048). In us, one product / three: 12 x 256 x 256
-    // 102 / 116, 12 x 256 x 1024 136 / 170, 48 x 256 x 1024 242 / 339; above, 12 x 768 x 768 343 / 495.
+    // 92 / 105, 12 x 256 x 1024 124 / 153, 48 x 256 x 1024 265 / 364; above, 12 x 768 x 768 348 / 502.
     int largest = 0;
     for (int i = 0; i < t.n; ++i) largest = std::max(largest, t.e[i].mp);
     const bool pairs = wt != DType::BF16 || largest <= 256;
