@@ -342,7 +342,7 @@ __device__ __forceinline__ int place_of_block() {
 //
 // What bounds it, 2 x 4096 x 4096: the matrix cores under the card's power limit. P X with three products runs at 1230
 // TFLOP/s issued (670 us), where the library's fp16 product of 8192^3 reaches 1170; with one product 905
-// (304 us). 12 x 768 x 768, 10 to 15 GFLOP a stage: 19 to 30 us, of which 9 do not depend on the length of the sum, the
+// (304 us). 12 x 768 x 768, 10 to 15 GFLOP a stage: 18 to 27 us, of which 9 do not depend on the length of the sum, the
 // start of a launch and the results on their way to memory behind it (14 to 28 MB: without the stores 12 to 25 us).
 template<int KIND, int BM, int BN, int WV, int KG, int ST, bool SPLIT, bool PAIRS, DType W>
 __global__ __launch_bounds__(64 * WV * KG, KG == 1 ? 2 : 4) void k_muon_product(MuonTable t, MuonStage st) {
