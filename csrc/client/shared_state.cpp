@@ -358,8 +358,8 @@ bool Client::sync_shared_state(SharedState &ss, SSInfo &info) {
                 break;
             }
             if (!be) {
-                LOG(ERR) << "Shared state sync: IPC entry " << se.key << " but no HIP backend";
-                ok = false;
+                LOG(WARN) << "Shared state sync: IPC entry " << se.key << " but no HIP backend; fetching over TCP";
+                fallback = true;
                 break;
             }
             DevPtrInfo pi{};
@@ -389,9 +389,18 @@ bool Client::sync_shared_state(SharedState &ss, SSInfo &info) {
                     } else {
                         VmmHandle vh;
                         int vfd = -1;
-                        if (VmmHandle::decode(hs[j], vh) && (vfd = VmmShare::fetch(vh.pid, vh.nonce, vh.id)) >= 0) {
+                        if (!VmmHandle::decode(hs[j], vh)) {
+                            LOG(WARN) << "Shared state sync: " << se.key << " has a malformed share handle";
+                        } else if ((vfd = VmmShare::fetch(vh.pid, vh.nonce, vh.id)) < 0) {
+                            LOG(WARN) << "Shared state sync: process " << vh.pid << " did not hand over the share of "
+                                      << se.key;
+                        } else {
                             m = be->vmm_import(vfd, vh.size, dev);
                             ::close(vfd);
+                            if (!m) {
+                                LOG(WARN) << "Shared state sync: the share of " << se.key << " cannot be mapped ("
+                                          << be->vmm_import_error() << ")";
+                            }
                         }
                         if (m) {
                             mapped.push_back({m, true, dev});
@@ -405,10 +414,16 @@ bool Client::sync_shared_state(SharedState &ss, SSInfo &info) {
                     srcs[i].push_back(static_cast<const uint8_t *>(m) + (j == 0 ? se.offset : 0));
                 }
             }
-            if (srcs[i].empty()) {
-                LOG(ERR) << "Shared state sync: cannot map the distributor's copy of " << se.key;
-                ok = false;
+            if (srcs[i].empty()) { // nothing has been copied yet: the distributor can still send every entry
+                LOG(WARN) << "Shared state sync: cannot map the distributor's copy of " << se.key
+                          << "; fetching over TCP";
+                fallback = true;
+                break;
             }
+        }
+        if (fallback) {
+            net::send_packet(fd, C2SSharedStateIpcDone{false});
+            return false;
         }
         if (const size_t ms = env_size("PCCL_SS_COPY_DELAY_MS", 0)) // tests: let the distributor die in between
             std::this_thread::sleep_for(std::chrono::milliseconds(ms));

@@ -57,6 +57,8 @@ public:
     virtual void vmm_free(void *p) = 0;                                // exporter side: unmap + release
     virtual void *vmm_import(int fd, size_t size, int device) = 0;    // importer side (does not take the fd)
     virtual void vmm_unmap(void *p) = 0;                               // importer side
+    // the step at which this thread's last vmm_import ended without a mapping, and its error
+    virtual const char *vmm_import_error() { return ""; }
     // allocation containing `p` (IPC handles always map the allocation base; offsets travel separately)
     virtual bool address_range(const void *p, void **base, size_t *size) = 0;
 

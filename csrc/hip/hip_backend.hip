@@ -191,7 +191,13 @@ public:
     void *vmm_import(int fd, size_t size, int device) override {
         hipMemGenericAllocationHandle_t h{};
         int fd_copy = fd; // the runtime takes a pointer to the fd
-        if (!HIP_OK(hipMemImportFromShareableHandle(&h, &fd_copy, hipMemHandleTypePosixFileDescriptor))) return nullptr;
+        const auto failed = [](const char *step, hipError_t e) {
+            std::snprintf(import_error_, sizeof(import_error_), "%s: %s", step, hipGetErrorString(e));
+            (void)hipGetLastError();
+            return nullptr;
+        };
+        const hipError_t e = hipMemImportFromShareableHandle(&h, &fd_copy, hipMemHandleTypePosixFileDescriptor);
+        if (e != hipSuccess) return failed("import", e);
         hipMemAllocationProp prop = vmm_prop(device);
         size_t gran = 0;
         if (!HIP_OK(hipMemGetAllocationGranularity(&gran, &prop, hipMemAllocationGranularityMinimum)) || gran == 0) {
@@ -199,6 +205,7 @@ public:
             return nullptr;
         }
         void *p = vmm_map(h, size, device, gran);
+        if (!p) failed("map", hipPeekAtLastError());
         (void)hipMemRelease(h); // the mapping keeps the physical memory alive (even after the exporter's death)
         if (!p) return nullptr;
         std::lock_guard l(vmm_mtx_);
@@ -206,6 +213,7 @@ public:
         return p;
     }
     void vmm_unmap(void *p) override { vmm_free(p); }
+    const char *vmm_import_error() override { return import_error_; }
     bool address_range(const void *p, void **base, size_t *size) override {
         hipDeviceptr_t b = nullptr;
         size_t n = 0;
@@ -404,6 +412,7 @@ private:
         bool owns_handle = false;
         int device = 0;
     };
+    static inline thread_local char import_error_[128] = "";
     std::mutex vmm_mtx_;
     std::map<void *, VmmMap> vmm_;
     std::map<void *, VmmMap> retained_; // freed exported allocations kept mapped for reuse

@@ -9,7 +9,10 @@
 // stream. Device memory is host memory: allocations of this backend are "device" pointers, and with
 // PCCL_HOSTDEV_ALL_DEVICE=1 every pointer is (a test's own buffers then take the device paths). Copies and the
 // reduce, quantize and de-quantize kernels run on the stream's thread with the host kernels (bit-identical to the HIP
-// kernels). The xGMI / IPC and VMM entry points report failure, so the library uses the TCP rings.
+// kernels). The xGMI / IPC entry points report failure, so the library uses the TCP rings. So do the VMM ones, unless
+// PCCL_HOSTDEV_VMM is set: shared memory files then take the part of shareable device memory (the shared state's
+// same-host hand-off). PCCL_HOSTDEV_VMM=no_import: a share of another process cannot be mapped, as on a machine whose
+// driver refuses it.
 //
 // Extra entry points for tests (dlsym): pccl_hostdev_fill(stream, ptr, n_floats, value, delay_us) queues a "producer
 // kernel" that sleeps delay_us, then writes `value` into n fp32 elements - input the stream-ordered ops must wait for;
@@ -26,6 +29,9 @@
 #include <memory>
 #include <mutex>
 #include <thread>
+
+#include <sys/mman.h>
+#include <unistd.h>
 
 #include "../common/device_backend.hpp"
 #include "../kernels/host_kernels.hpp"
@@ -142,10 +148,34 @@ public:
     bool ipc_export(void *, uint8_t *) override { return false; }
     void *ipc_open(const uint8_t *) override { return nullptr; }
     void ipc_close(void *) override {}
-    void *vmm_alloc(size_t, int, int *, size_t *) override { return nullptr; }
-    void vmm_free(void *) override {}
-    void *vmm_import(int, size_t, int) override { return nullptr; }
-    void vmm_unmap(void *) override {}
+    void *vmm_alloc(size_t n, int, int *fd_out, size_t *alloc_size) override {
+        if (!vmm_) return nullptr;
+        const size_t size = (std::max<size_t>(n, 1) + 4095) / 4096 * 4096;
+        const int fd = ::memfd_create("pccl-hostdev", MFD_CLOEXEC);
+        if (fd < 0) return nullptr;
+        void *p = ::ftruncate(fd, static_cast<off_t>(size)) == 0 ? vmm_map(fd, size) : nullptr;
+        if (!p) {
+            ::close(fd);
+            return nullptr;
+        }
+        *fd_out = fd;
+        *alloc_size = size;
+        return p;
+    }
+    void vmm_free(void *p) override {
+        size_t size = 0;
+        {
+            std::lock_guard l(alloc_m_);
+            auto it = allocs_.find(reinterpret_cast<uintptr_t>(p));
+            if (it == allocs_.end()) return;
+            size = it->second;
+            allocs_.erase(it);
+        }
+        ::munmap(p, size);
+    }
+    void *vmm_import(int fd, size_t size, int) override { return vmm_ && vmm_imports_ ? vmm_map(fd, size) : nullptr; }
+    void vmm_unmap(void *p) override { vmm_free(p); }
+    const char *vmm_import_error() override { return "emulated refusal"; }
     bool address_range(const void *p, void **base, size_t *size) override {
         std::lock_guard l(alloc_m_);
         auto it = allocs_.upper_bound(reinterpret_cast<uintptr_t>(p));
@@ -289,9 +319,14 @@ public:
                       bool) override {
         return false;
     }
-    bool multi_gather(void *, const void *const *, const size_t *, const size_t *, int, int, DType, DevStream,
-                      bool) override {
-        return false;
+    bool multi_gather(void *dst, const void *const *srcs, const size_t *offsets, const size_t *counts, int n, int skip,
+                      DType t, DevStream s, bool) override {
+        if (!vmm_) return false;
+        for (int k = 0; k < n; ++k)
+            if (k != skip)
+                memcpy_async(static_cast<uint8_t *>(dst) + offsets[k] * dtype_size(t), srcs[k],
+                             counts[k] * dtype_size(t), s);
+        return true;
     }
     uint32_t simplehash(const void *p, size_t n, DevStream s) override {
         stream_of(s)->sync();
@@ -325,7 +360,16 @@ private:
         size_t n;
         return address_range(p, &b, &n);
     }
+    void *vmm_map(int fd, size_t size) {
+        void *p = ::mmap(nullptr, size, PROT_READ | PROT_WRITE, MAP_SHARED, fd, 0);
+        if (p == MAP_FAILED) return nullptr;
+        std::lock_guard l(alloc_m_);
+        allocs_[reinterpret_cast<uintptr_t>(p)] = size;
+        return p;
+    }
     const bool all_device_;
+    const bool vmm_ = std::getenv("PCCL_HOSTDEV_VMM") != nullptr;
+    const bool vmm_imports_ = vmm_ && std::strcmp(std::getenv("PCCL_HOSTDEV_VMM"), "no_import") != 0;
     std::atomic<Stream *> null_stream_{nullptr};
     std::mutex alloc_m_;
     std::map<uintptr_t, size_t> allocs_;
