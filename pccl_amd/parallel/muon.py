@@ -46,7 +46,7 @@ class Muon(torch.optim.Optimizer):
         return params if params and isinstance(params[0], dict) else [{"params": params}] if params else []
 
     def add_param_group(self, param_group: Dict[str, Any]) -> None:
-        if not param_group.get("muon", True) and "betas" not in param_group:
+        if not param_group.get("muon", True) and hasattr(self, "_adamw"):
             raise ValueError("Muon: parameters for AdamW are given to the constructor")
         super().add_param_group(param_group)
         group = self.param_groups[-1]

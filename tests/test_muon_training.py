@@ -352,3 +352,22 @@ def test_sharded_example_refuses_muon():
     r = subprocess.run([sys.executable, os.path.join(EX, "sync_diloco_fsdp.py"), "--optimizer", "muon"],
                        capture_output=True, text=True, timeout=120)
     assert r.returncode == 2 and "whole matrices" in r.stderr
+
+
+def test_added_group_for_adamw_is_refused(device):
+    """Parameters that no part of the optimizer would update are not taken, whatever settings come with them."""
+    params = small_params(device)
+    like_torch = torch.optim.AdamW(params[3:], lr=0.1).param_groups[0]
+    for others in ([], params[2:3]):
+        opt = Muon(params[:1], others, lr=0.1)
+        groups = len(opt.param_groups)
+        for settings in (dict(betas=(0.9, 0.95)), {k: v for k, v in like_torch.items() if k != "params"}):
+            with pytest.raises(ValueError, match="constructor"):
+                opt.add_param_group({"params": params[3:], "muon": False, **settings})
+        opt.add_param_group({"params": params[1:2]})
+        assert len(opt.param_groups) == groups + 1
+        fill_grads(params, 0)
+        before = copy.deepcopy([p.detach() for p in params])
+        opt.step()
+        held = {id(p) for g in opt.param_groups for p in g["params"]}
+        assert [torch.equal(p, q) for p, q in zip(params, before)] == [id(p) not in held for p in params]
