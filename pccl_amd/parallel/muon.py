@@ -63,6 +63,12 @@ class Muon(torch.optim.Optimizer):
             self.param_groups.pop()
             raise
 
+    def __setstate__(self, state: Dict[str, Any]) -> None:
+        """A copy, an unpickled optimizer or one that loaded a checkpoint: the AdamW part follows from the groups."""
+        super().__setstate__(state)
+        others = [g for g in self.param_groups if not g["muon"]]
+        self._adamw = torch.optim.AdamW(others) if others else None
+
     def load_state_dict(self, state_dict: Dict[str, Any]) -> None:
         super().load_state_dict(state_dict)  # casts state to the parameter's type; the momentum stays fp32
         saved = state_dict["state"]

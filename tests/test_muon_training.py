@@ -7,6 +7,7 @@ E = (2 V / 64 + 64) 2^-24 (1 + ln V)), of Muon steps those of tests/test_muon.py
 import copy
 import math
 import os
+import pickle
 import subprocess
 import sys
 
@@ -371,3 +372,38 @@ def test_added_group_for_adamw_is_refused(device):
         opt.step()
         held = {id(p) for g in opt.param_groups for p in g["params"]}
         assert [torch.equal(p, q) for p, q in zip(params, before)] == [id(p) not in held for p in params]
+
+
+@pytest.mark.parametrize("how", ["deepcopy", "pickle", "load"])
+@pytest.mark.parametrize("with_others", [True, False])
+def test_copies_go_on_alike(device, how, with_others):
+    """A copied or unpickled optimizer, and one that takes over another's groups with its state, steps to equal bits."""
+    params = small_params(device)
+    take = params if with_others else params[:2]
+    opt = Muon([{"params": params[:1], "lr": 0.05}, {"params": params[1:2], "nesterov": False}],
+               [{"params": params[2:3], "weight_decay": 0.0}, {"params": params[3:]}] if with_others else [], lr=0.02,
+               betas=(0.8, 0.9), fused=device.type == "cuda")
+    for turn in range(2):
+        fill_grads(params, turn)
+        opt.step()
+    if how == "deepcopy":
+        copied, again = copy.deepcopy((take, opt))
+    elif how == "pickle":
+        copied, again = pickle.loads(pickle.dumps((take, opt)))
+    else:
+        copied = [p.detach().clone().requires_grad_() for p in take]
+        # groups of matrices only: which part a group belongs to comes with the state
+        again = Muon([{"params": [p.view(-1, 1).detach().requires_grad_()] if p.dim() == 1 else [p]} for p in copied])
+        for g, p in zip(again.param_groups, copied):
+            g["params"] = [p]
+        again.load_state_dict(copy.deepcopy(opt.state_dict()))
+    assert [g["muon"] for g in again.param_groups] == [True, True, False, False][:len(take)]
+    for turn in range(2, 4):
+        for ps, o in ((params, opt), (copied, again)):
+            fill_grads(ps, turn)
+            o.step()
+    assert all(torch.equal(p, q) for p, q in zip(take, copied))
+    assert all(p is not q for p, q in zip(take, copied))
+    for p, q in zip(take, copied):
+        for k, v in opt.state[p].items():
+            assert again.state[q][k].dtype == v.dtype and torch.equal(again.state[q][k], v), k
