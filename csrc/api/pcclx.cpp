@@ -260,17 +260,32 @@ PCCLX_EXPORT int pcclxOuterSgd(float *outer, float *mom, const float *pg, void *
     return be->outer_sgd(outer, mom, pg, local, count, lt, p, nullptr) && be->device_sync() ? 0 : -1;
 }
 
+namespace {
+
+// types of the logits, of a matrix
+bool float_type(int dtype) {
+    return dtype == static_cast<int>(DType::F32) || dtype == static_cast<int>(DType::BF16) ||
+           dtype == static_cast<int>(DType::F16);
+}
+
+bool logprob_sizes_ok(int64_t rows, int64_t vocab, int dtype, int top_k) {
+    return rows >= 0 && rows <= INT32_MAX && vocab >= 1 && vocab <= INT32_MAX && float_type(dtype) && top_k >= 0 &&
+           top_k <= kernels::kMaxTopLogprobs && top_k <= vocab;
+}
+
+} // namespace
+
 // Log probabilities of given tokens (csrc/kernels/logprob_common.hpp), asynchronous on `stream` of the current device.
 // Returns 0, -1 (no device backend, or the launch failed) or -2 (arguments).
 PCCLX_EXPORT int pcclxTokenLogprobs(const void *logits, int64_t row_stride, int64_t rows, int64_t vocab, int dtype,
                                     const int64_t *targets, int64_t ignore_index, int top_k, float *logprob,
                                     float *entropy, float *stats, float *top_logprob, int64_t *top_index,
                                     void *stream) {
+    if (!logprob_sizes_ok(rows, vocab, dtype, top_k) ||
+        (rows && (!logits || !targets || !logprob || !entropy || !stats || (top_k && (!top_logprob || !top_index)))))
+        return -2;
     DeviceBackend *be = device_backend();
     if (!be) return -1;
-    if (rows < 0 || rows > INT32_MAX || vocab < 1 || vocab > INT32_MAX || top_k < 0 ||
-        top_k > kernels::kMaxTopLogprobs || top_k > vocab || (rows && (!logits || !targets)))
-        return -2;
     const kernels::LogprobArgs a{logits,  row_stride, rows,  vocab,       targets,  ignore_index,
                                  top_k,   logprob,    entropy, stats, top_logprob, top_index};
     return be->token_logprobs(a, static_cast<DType>(dtype), stream) ? 0 : -1;
@@ -282,11 +297,11 @@ PCCLX_EXPORT int pcclxTokenLogprobsGrad(const void *logits, int64_t row_stride, 
                                         const float *stats, const int64_t *top_index,
                                         const float *g_logprob, const float *g_entropy, const float *g_top,
                                         void *d_logits, void *stream) {
+    if (!logprob_sizes_ok(rows, vocab, dtype, top_k) ||
+        (rows && (!logits || !targets || !stats || !d_logits || (top_k && g_top && !top_index))))
+        return -2;
     DeviceBackend *be = device_backend();
     if (!be) return -1;
-    if (rows < 0 || rows > INT32_MAX || vocab < 1 || vocab > INT32_MAX || top_k < 0 ||
-        top_k > kernels::kMaxTopLogprobs || top_k > vocab || (rows && (!logits || !targets || !stats || !d_logits)))
-        return -2;
     kernels::LogprobGradArgs g;
     g.fwd = {logits, row_stride, rows, vocab, targets, ignore_index, top_k, nullptr, nullptr,
              const_cast<float *>(stats), nullptr, const_cast<int64_t *>(top_index)};
@@ -302,9 +317,12 @@ namespace {
 // entries of a call: shapes[3 i ..] = count, rows, cols; false if a size is out of range
 bool muon_entries(int n, const int64_t *shapes, std::vector<kernels::MuonEntry> &out) {
     constexpr int64_t kMax = INT32_MAX - kernels::kMuonPad;
+    constexpr int64_t kMaxElems = int64_t{1} << 56; // of one entry: no address space holds it, and bytes stay in range
+    if (n > 0 && !shapes) return false;
     for (int i = 0; i < n; ++i) {
         const int64_t count = shapes[3 * i], rows = shapes[3 * i + 1], cols = shapes[3 * i + 2];
         if (count < 0 || rows < 0 || cols < 0 || count > kMax || rows > kMax || cols > kMax) return false;
+        if (rows && cols && count > kMaxElems / rows / cols) return false;
         kernels::MuonEntry e;
         e.count = static_cast<int>(count);
         e.rows = static_cast<int>(rows);
@@ -354,8 +372,9 @@ PCCLX_EXPORT int pcclxMuon(int n, const int64_t *shapes, const void *const *g, i
                            void *stream) {
     try {
         const auto gt = static_cast<DType>(gtype), wt = static_cast<DType>(wtype);
-        const auto ok_type = [](DType t) { return t == DType::F32 || t == DType::BF16 || t == DType::F16; };
-        if (n < 0 || steps < 1 || !ok_type(gt) || !ok_type(wt)) return -2;
+        if (n < 0 || steps < 1 || !float_type(gtype) || !float_type(wtype) || !coefficients || (n > 0 && (!g || !w)) ||
+            (mom && !alpha))
+            return -2;
         std::vector<kernels::MuonEntry> entries;
         if (!muon_entries(n, shapes, entries)) return -2;
         std::vector<Span> spans;
@@ -380,7 +399,7 @@ PCCLX_EXPORT int pcclxMuon(int n, const int64_t *shapes, const void *const *g, i
         if (spans_collide(spans)) return -3;
         std::vector<std::vector<kernels::MuonEntry>> groups;
         const size_t need = kernels::muon_plan(entries, dtype_size(gt), dtype_size(wt), &groups);
-        if (workspace_bytes < 0 || static_cast<size_t>(workspace_bytes) < need ||
+        if (workspace_bytes < 0 || static_cast<size_t>(workspace_bytes) < need || (need > 0 && !workspace) ||
             reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
             return -2;
         if (groups.empty()) return 0;
