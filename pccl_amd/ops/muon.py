@@ -17,7 +17,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from .._native import C
-from ._launch import on_device, refuse_tangents, require_hip, stream_of
+from ._launch import on_device, require_hip, stream_of
 from .kernels import WIRE_DTYPE, _check
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
@@ -85,11 +85,11 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence[flo
     """The orthogonal factor of each matrix of ``x`` ([..., m, n], fp32 / bf16 / fp16), by ``steps`` Newton-Schulz
     steps from ``x / max(||x||_F, eps)``; singular values end near 1, in about [0.7, 1.2] with the default coefficients.
 
-    Not differentiable (a GPU tensor with a forward-mode tangent is refused). The norm is summed in 64 bits; an fp32 or fp16 result has the error of fp32 products, a bf16
+    Not differentiable. The norm is summed in 64 bits; an fp32 or fp16 result has the error of fp32 products, a bf16
     result one rounding more than bf16's own. A zero matrix gives zero, one with a NaN or an infinity gives NaN.
     Non-contiguous input is copied. ``out`` (contiguous, of x's shape and type) may be ``x`` itself.
     """
-    coefficients, steps = tuple(map(float, coefficients)), index(steps)
+    coefficients, steps = tuple(coefficients), index(steps)
     _check_coefficients(coefficients, steps)
     if x.dim() < 2:
         raise ValueError(f"orthogonalize: a matrix or a stack of them, got shape {tuple(x.shape)}")
@@ -111,7 +111,6 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence[flo
         return out.copy_(_host_orthogonalize(x, steps, coefficients, eps))
     if x.device.type != "cuda":
         raise ValueError(f"orthogonalize: no kernel for device {x.device}")
-    refuse_tangents("orthogonalize", x, out)
     m, n = x.shape[-2:]
     x = x.contiguous()
     _queue((x.numel() // (m * n), m, n), (x.data_ptr(),), x.dtype, (out.data_ptr(),), x.dtype, None, None, 1.0, 0.0, 0,
@@ -131,8 +130,8 @@ def _shape_factor(rows: int, cols: int, adjust_lr: str) -> float:
 
 
 def check_muon(what: str, lr: float, weight_decay: float, momentum: float, steps: int,
-               coefficients: Sequence[float], eps: float, adjust_lr: str) -> None:
-    _check_coefficients(tuple(map(float, coefficients)), steps)
+               coefficients: Tuple[float, ...], eps: float, adjust_lr: str) -> None:
+    _check_coefficients(coefficients, steps)
     if not eps > 0 or not math.isfinite(eps):
         raise ValueError(f"{what}: eps must be positive, got {eps}")
     if not 0.0 <= momentum <= 1.0:
@@ -159,7 +158,7 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     memory with another (a parameter listed twice is refused; a gradient may serve several parameters). Equal calls give
     equal bits on every peer. The call may be captured into a graph, which then keeps its learning rate.
     """
-    coefficients, steps = tuple(map(float, coefficients)), index(steps)
+    coefficients, steps = tuple(coefficients), index(steps)
     check_muon("muon_step", lr, weight_decay, momentum, steps, coefficients, eps, adjust_lr)
     if not len(params) == len(grads) == len(momentum_buffers):
         raise ValueError(f"muon_step: {len(params)} parameters, {len(grads)} gradients and {len(momentum_buffers)} "
@@ -197,7 +196,6 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     alpha = [factors[e[:2]] for e in work]
     decay = 1.0 - lr * weight_decay
     if device.type == "cuda":
-        refuse_tangents("muon_step", *(t for e in work for t in e[2:]))
         _queue([v for e in work for v in (1, e[0], e[1])], [e[3].data_ptr() for e in work], gtype,
                [e[2].data_ptr() for e in work], wtype, [e[4].data_ptr() for e in work], alpha, decay, momentum,
                int(nesterov), steps, coefficients, eps, device, "muon_step")
