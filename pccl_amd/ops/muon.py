@@ -89,7 +89,7 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence[flo
     result one rounding more than bf16's own. A zero matrix gives zero, one with a NaN or an infinity gives NaN.
     Non-contiguous input is copied. ``out`` (contiguous, of x's shape and type) may be ``x`` itself.
     """
-    coefficients, steps = tuple(coefficients), index(steps)
+    coefficients, steps = tuple(map(float, coefficients)), index(steps)
     _check_coefficients(coefficients, steps)
     if x.dim() < 2:
         raise ValueError(f"orthogonalize: a matrix or a stack of them, got shape {tuple(x.shape)}")
@@ -130,8 +130,8 @@ def _shape_factor(rows: int, cols: int, adjust_lr: str) -> float:
 
 
 def check_muon(what: str, lr: float, weight_decay: float, momentum: float, steps: int,
-               coefficients: Tuple[float, ...], eps: float, adjust_lr: str) -> None:
-    _check_coefficients(coefficients, steps)
+               coefficients: Sequence[float], eps: float, adjust_lr: str) -> None:
+    _check_coefficients(tuple(map(float, coefficients)), steps)
     if not eps > 0 or not math.isfinite(eps):
         raise ValueError(f"{what}: eps must be positive, got {eps}")
     if not 0.0 <= momentum <= 1.0:
@@ -158,7 +158,7 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     memory with another (a parameter listed twice is refused; a gradient may serve several parameters). Equal calls give
     equal bits on every peer. The call may be captured into a graph, which then keeps its learning rate.
     """
-    coefficients, steps = tuple(coefficients), index(steps)
+    coefficients, steps = tuple(map(float, coefficients)), index(steps)
     check_muon("muon_step", lr, weight_decay, momentum, steps, coefficients, eps, adjust_lr)
     if not len(params) == len(grads) == len(momentum_buffers):
         raise ValueError(f"muon_step: {len(params)} parameters, {len(grads)} gradients and {len(momentum_buffers)} "

@@ -15,7 +15,7 @@ import pytest
 import torch
 
 from pccl_amd.models import GPT, GPTConfig
-from pccl_amd.ops import muon_step, token_logprobs
+from pccl_amd.ops import muon_step, orthogonalize, token_logprobs
 from pccl_amd.parallel import Muon, init_optimizer_state, state_tensors
 from test_examples import EX, _run
 from test_logprobs import close, sum_error
@@ -407,3 +407,27 @@ def test_copies_go_on_alike(device, how, with_others):
     for p, q in zip(take, copied):
         for k, v in opt.state[p].items():
             assert again.state[q][k].dtype == v.dtype and torch.equal(again.state[q][k], v), k
+
+
+def test_coefficients_of_a_group_and_as_tensors(device):
+    """Any sequence of three numbers; what tensors among them hold is read anew by every call."""
+    x = gradient((20, 30), 1, device)
+    abc = torch.tensor([1.5, -0.5, 0.0], dtype=torch.float64)
+    first = orthogonalize(x, coefficients=abc.unbind())
+    assert torch.equal(first, orthogonalize(x, coefficients=[1.5, -0.5, 0.0]))
+    numbers = abc.unbind()
+    orthogonalize(x, coefficients=numbers)
+    abc.copy_(torch.tensor([1.875, -1.25, 0.375]))
+    assert torch.equal(orthogonalize(x, coefficients=numbers), orthogonalize(x, coefficients=(1.875, -1.25, 0.375)))
+    abc[0] = 9.0
+    with pytest.raises(ValueError, match="coefficients"):
+        orthogonalize(x, coefficients=numbers)
+    params = small_params(device)[:2]
+    opt = Muon([{"params": params[:1], "coefficients": [1.5, -0.5, 0.0]}, {"params": params[1:]}], lr=0.1,
+               coefficients=[1.875, -1.25, 0.375])
+    fill_grads(params, 0)
+    want = [(p.detach().clone(), torch.zeros_like(p)) for p in params]
+    opt.step()
+    for p, (q, b), c in zip(params, want, ((1.5, -0.5, 0.0), (1.875, -1.25, 0.375))):
+        muon_step([q], [p.grad], [b], lr=0.1, adjust_lr="match_rms_adamw", coefficients=c)
+        assert torch.equal(p, q)
