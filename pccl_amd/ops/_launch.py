@@ -16,6 +16,12 @@ def require_hip() -> None:
         raise RuntimeError("pccl-amd HIP backend (libpccl_hip.so) is not loaded but a GPU tensor was passed")
 
 
+def refuse_inference(what: str, *written: torch.Tensor) -> None:
+    """torch lets nothing write an inference tensor outside of inference mode; asked before anything is written."""
+    if any(t.is_inference() for t in written) and not torch.is_inference_mode_enabled():
+        raise RuntimeError(f"{what}: an inference tensor would be written outside of inference mode")
+
+
 def on_device(device: torch.device):
     """A context in which ``device`` is the current one (the kernels are launched on the current device)."""
     return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)

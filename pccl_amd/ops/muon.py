@@ -17,7 +17,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from .._native import C
-from ._launch import on_device, require_hip, stream_of
+from ._launch import on_device, refuse_inference, require_hip, stream_of
 from .kernels import WIRE_DTYPE, _check
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
@@ -105,6 +105,7 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence[flo
         raise ValueError("orthogonalize: out must be contiguous and match x in shape, type and device")
     elif torch.is_grad_enabled() and out.requires_grad:
         raise RuntimeError("orthogonalize: out requires a gradient: call it under no_grad")
+    refuse_inference("orthogonalize", out)
     if x.numel() == 0:
         return out
     if x.device.type == "cpu":
@@ -189,6 +190,7 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
             work.append((rows, cols, p, g if g.is_contiguous() else g.detach().contiguous(), b))
     if not work:
         return
+    refuse_inference("muon_step", *(t for e in work for t in (e[2], e[4])))
     factors = {}
     for e in work:
         if e[:2] not in factors:
