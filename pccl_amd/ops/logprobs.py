@@ -193,6 +193,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top_k: int = 
         raise ValueError(f"token_logprobs: targets on {targets.device}, logits on {logits.device}")
     if not 0 <= top_k <= min(MAX_TOP_LOGPROBS, logits.shape[-1]):
         raise ValueError(f"token_logprobs: top_k {top_k} is not in 0..{min(MAX_TOP_LOGPROBS, logits.shape[-1])}")
+    if not -1 << 63 <= ignore_index < 1 << 63:  # the kernels would take it modulo 2^64
+        raise ValueError(f"token_logprobs: ignore_index {ignore_index} is no int64")
     if targets.numel() >= 1 << 31 or logits.shape[-1] >= 1 << 31:
         raise ValueError("token_logprobs: at most 2^31 - 1 rows and tokens of vocabulary")
     if logits.device.type == "cuda":

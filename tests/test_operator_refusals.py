@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from pccl_amd.ops import muon_step, orthogonalize
+from pccl_amd.ops import muon_step, orthogonalize, token_logprobs
 from test_muon import gradient
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
@@ -32,3 +32,14 @@ def test_inference_tensors(device):
         muon_step([q], [g], [c], lr=0.1)
         assert torch.equal(orthogonalize(x, out=out), orthogonalize(x))
         assert torch.equal(q, p) and torch.equal(c, b)
+
+
+def test_ignore_index_is_a_token(device):
+    """2^64 - 100 is not -100."""
+    x, t = gradient((6, 5), 1, device), torch.full((6,), -100, device=device)
+    for bad in ((1 << 64) - 100, 1 << 63, -(1 << 63) - 1):
+        with pytest.raises(ValueError, match="ignore_index"):
+            token_logprobs(x, t, ignore_index=bad)
+    for fine in ((1 << 63) - 1, -(1 << 63)):
+        assert bool(token_logprobs(x, t, ignore_index=fine).logprob.isnan().all())
+        assert not token_logprobs(x, torch.full_like(t, fine), ignore_index=fine).logprob.any()
