@@ -172,6 +172,6 @@ class GPT(nn.Module):
                 logprobs.append(token_logprobs(raw, token[:, 0]).logprob)
             idx = torch.cat((idx, token), dim=1)
         if return_logprobs:
-            none = torch.zeros((idx.size(0), 0), device=idx.device)
+            none = torch.zeros((idx.size(0), 0), dtype=torch.float32, device=idx.device)
             return idx, torch.stack(logprobs, dim=1) if logprobs else none
         return idx

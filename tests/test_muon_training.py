@@ -431,3 +431,13 @@ def test_coefficients_of_a_group_and_as_tensors(device):
     for p, (q, b), c in zip(params, want, ((1.5, -0.5, 0.0), (1.875, -1.25, 0.375))):
         muon_step([q], [p.grad], [b], lr=0.1, adjust_lr="match_rms_adamw", coefficients=c)
         assert torch.equal(p, q)
+
+
+def test_no_generated_token_has_fp32_logprobs(device):
+    model, idx, _ = make(SIZES[0], device)
+    kept = torch.get_default_dtype()
+    torch.set_default_dtype(torch.float64)
+    try:
+        assert model.generate(idx, 0, return_logprobs=True)[1].dtype == torch.float32
+    finally:
+        torch.set_default_dtype(kept)
