@@ -166,7 +166,8 @@ bool MuxConn::send_frame(uint64_t tag, uint64_t ctr, const void *data, size_t n)
     // bulk frames from pinned staging buffers may go out as MSG_ZEROCOPY (socket.cpp: sendv_all_zerocopy)
     const bool zc = zerocopy_ && n >= (256u << 10);
     send_since_ns_.store(steady_ns(), std::memory_order_relaxed);
-    const bool ok = zc ? sendv_all_zerocopy(fd_, iov, n ? 2 : 1, zc_next_id_) : sendv_all(fd_, iov, n ? 2 : 1);
+    const bool ok = zc ? sendv_all_zerocopy(fd_, iov, n ? 2 : 1, zc_next_id_, zerocopy_) : sendv_all(fd_, iov, n ? 2 : 1);
+    if (zc && !zerocopy_) LOG(INFO) << "MuxConn: memory that the kernel cannot pin, plain sends from here on";
     send_since_ns_.store(0, std::memory_order_relaxed);
     if (!ok) {
         open_.store(false, std::memory_order_release);

@@ -225,24 +225,30 @@ bool sendv_all(int fd, iovec *iov, int iovcnt) {
 // user pages instead of copying them into socket buffers and reports completion on the socket's error queue; the call returns once every
 // byte it sent is released, so the caller may reuse the buffer as after a plain send. On loopback the kernel copies
 // the pages anyway when it delivers them to the receiving socket ("deferred copy", reported as
-// SO_EE_CODE_ZEROCOPY_COPIED), so only a real NIC saves the copy. Returns false on error.
-bool sendv_all_zerocopy(int fd, iovec *iov, int iovcnt, uint32_t &next_id) {
+// SO_EE_CODE_ZEROCOPY_COPIED), so only a real NIC saves the copy. Memory without pages of its own that the kernel may
+// pin (what some GPU drivers map for pinned host allocations) goes out as plain sends. Returns false on error.
+bool sendv_all_zerocopy(int fd, iovec *iov, int iovcnt, uint32_t &next_id, bool &pinnable) {
     uint32_t first = next_id;
     bool sent_any = false;
     while (iovcnt > 0) {
         msghdr msg{};
         msg.msg_iov = iov;
         msg.msg_iovlen = static_cast<size_t>(iovcnt);
-        ssize_t k = ::sendmsg(fd, &msg, MSG_NOSIGNAL | MSG_ZEROCOPY);
+        const bool zc = pinnable;
+        ssize_t k = ::sendmsg(fd, &msg, zc ? MSG_NOSIGNAL | MSG_ZEROCOPY : MSG_NOSIGNAL);
         if (k < 0) {
             if (errno == EINTR) continue;
-            if (errno == ENOBUFS) { // optmem exhausted by pinned pages in flight: fall back for this piece
+            if (zc && errno == EFAULT) { // unreadable memory fails the plain send as well
+                pinnable = false;
+                continue;
+            }
+            if (zc && errno == ENOBUFS) { // optmem exhausted by pinned pages in flight: fall back for this piece
                 k = ::sendmsg(fd, &msg, MSG_NOSIGNAL);
                 if (k < 0) return false;
             } else {
                 return false;
             }
-        } else {
+        } else if (zc) {
             ++next_id; // every successful MSG_ZEROCOPY call takes one notification id
             sent_any = true;
         }

@@ -5,7 +5,9 @@
 //   socket helpers   - blocking LTV / full send-recv / connect / listen (reference BlockingIOSocket)
 //   MuxConn          - the multiplexed P2P data connection (reference MultiplexedIOSocket)
 // Also run under the ASan/UBSan and TSan builds (tests/test_native.py).
+#include <sys/mman.h>
 #include <sys/socket.h>
+#include <sys/syscall.h>
 #include <unistd.h>
 
 #include <atomic>
@@ -706,4 +708,56 @@ TEST(mux_send_on_closed_connection_fails) {
     for (int k = 0; k < 64 && !failed; ++k) failed = !tx->send_frame(1, 1, p.data(), p.size());
     EXPECT(failed);
     delete tx;
+}
+
+// Memory that the kernel cannot pin for MSG_ZEROCOPY, as a GPU driver's mapping of pinned host memory may be: secret
+// memory refuses the pages and allows the copy.
+TEST(mux_sends_memory_that_cannot_be_pinned) {
+    const size_t n = 3u << 20;
+    const int mem = static_cast<int>(::syscall(447 /* memfd_secret */, 0));
+    void *p = mem >= 0 && ::ftruncate(mem, static_cast<off_t>(n)) == 0
+                  ? ::mmap(nullptr, n, PROT_READ | PROT_WRITE, MAP_SHARED, mem, 0)
+                  : MAP_FAILED;
+    if (p == MAP_FAILED) {
+        std::fprintf(stderr, "  skipped: no secret memory on this kernel\n");
+        if (mem >= 0) ::close(mem);
+        return;
+    }
+    auto *secret = static_cast<uint8_t *>(p);
+    std::vector<uint8_t> plain(n);
+    for (size_t i = 0; i < n; ++i) {
+        secret[i] = static_cast<uint8_t>(i * 7 + (i >> 12));
+        plain[i] = static_cast<uint8_t>(i * 5 + (i >> 11));
+    }
+    uint16_t port = 0;
+    const int lfd = net::listen_tcp(inetIPv4, 0, false, port);
+    const int tx = net::connect_tcp(loop_v4(port)), rx = ::accept(lfd, nullptr, nullptr);
+    EXPECT(tx >= 0 && rx >= 0);
+    net::tune_socket(tx, true);
+    EXPECT(net::socket_zerocopy_on(tx));
+    {
+        net::MuxConn conn(tx, net::MuxConn::Mode::Tx, loop_v4(port));
+        conn.start();
+        // zero-copy first, so that notifications are out when the memory is refused; then both kinds
+        const std::vector<const uint8_t *> frames{plain.data(), secret, plain.data(), secret};
+        std::thread reader([&] {
+            std::vector<uint8_t> got(24 + n);
+            for (const uint8_t *want : frames) {
+                EXPECT(net::recv_all(rx, got.data(), got.size()));
+                EXPECT(std::memcmp(got.data() + 24, want, n) == 0);
+            }
+        });
+        for (size_t k = 0; k < frames.size(); ++k) EXPECT(conn.send_frame(1, k, frames[k], n));
+        if (!conn.is_open()) ::shutdown(rx, SHUT_RDWR); // (a failed send: nothing more comes)
+        reader.join();
+    }
+    // memory that cannot be read at all is an error, not an endless retry
+    const int tx2 = net::connect_tcp(loop_v4(port)), rx2 = ::accept(lfd, nullptr, nullptr);
+    net::tune_socket(tx2, true);
+    iovec iov{secret, n};
+    ::munmap(p, n);
+    uint32_t id = 0;
+    bool pinnable = true;
+    EXPECT(!net::sendv_all_zerocopy(tx2, &iov, 1, id, pinnable));
+    for (int fd : {rx, rx2, tx2, lfd, mem}) ::close(fd);
 }
