@@ -398,3 +398,41 @@ def test_more_rows_than_a_launch_has(hip, top_k):
         got, want = got.detach(), want.detach()
         assert bool((got[:7 * n].view(n, 7, -1) == want.reshape(7, -1)).all())
         assert torch.equal(got[7 * n:], want[:rows - 7 * n])
+
+
+def edge_positions(vocab, width):
+    """Columns where a split of the row over threads, unrolled loads or blocks of `width` elements could lose or double
+    one: the ends, and both sides of every multiple of 4 x 64 .. 4 x 512 blocks and of the remainders behind them."""
+    at = set(range(min(vocab, 2 * width + 1))) | set(range(max(0, vocab - 3 * width), vocab))
+    for threads in (64, 128, 256, 512):
+        sweep = 4 * threads * width
+        for edge in [*range(sweep, vocab, sweep)][-2:] + [vocab // sweep * sweep + threads * width * k for k in range(4)]:
+            at |= {edge - 1, edge, edge + 1, edge + width - 1, edge + width}
+    return sorted(i for i in at if 0 <= i < vocab)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab,top_k", [(50257, 0), (50304, 2), (50257, 3), (9001, 3), (8191, 0), (4100, 2), (1023, 3),
+                                         (255, 0)])
+def test_every_element_counts_once(device, dtype, vocab, top_k):
+    """Rows of which two or three entries have all the mass, so that losing or doubling one shows. The sums then have
+    three terms, each off by at most 4 u and rounded twice."""
+    positions = edge_positions(vocab, 16 // dtype.itemsize)
+    n = len(positions)
+    at = torch.tensor([[p, (7 * p + 13) % vocab, vocab - 1 - p] for p in positions])
+    x = torch.full((n, vocab), -1e4)
+    x.scatter_(1, at, torch.tensor([1.0, 0.5, 0.0]).expand(n, 3))  # of equal places one counts
+    x = x.to(dtype)
+    targets = at[:, 0]
+    lp, entropy, top_lp, index, logp, p = reference(x, targets, top_k)
+    leaf = x.to(device).requires_grad_()
+    r = token_logprobs(leaf, targets.to(device), top_k=top_k)
+    close(r.logprob, lp, 32 * U)
+    close(r.entropy, entropy, 32 * U)
+    if top_k:
+        assert torch.equal(r.top_index[:, :2].cpu(), index[:, :2])
+        close(r.top_logprob[:, :2], top_lp[:, :2], 32 * U)
+    d, = torch.autograd.grad(r.logprob.sum(), leaf)
+    want = -p
+    want.scatter_add_(1, targets[:, None], torch.ones(n, 1, dtype=torch.float64))
+    close(d, want, want.abs() * torch.finfo(dtype).eps / 2 * 1.01 + 64 * U)
