@@ -6,10 +6,9 @@
 // a X + P X, whose last pass updates the caller's parameters instead of writing X. No atomics and a fixed order of
 // every sum: equal calls give equal bits, which the peers of a run rely on.
 //
-// The products of the 16-bit types: where the result is bf16 (8 bits) and the matrices are not small (launch_muon), A
-// and P X use the hi parts alone (11 bits) and only A A, the cheapest, all three; the term a X always has both parts, so
-// small singular values, which the steps amplify up to a^steps, keep their precision. Otherwise three products
-// everywhere, the error of fp32 products.
+// Every product is three of the 16-bit parts, the error of fp32 products, whatever the type of the result and whatever
+// else the call holds. (With one product of the hi parts for A and P X a bf16 result takes 0.5 to 0.7 of the time, but is
+// then up to 1.4 times as far off as its own rounding.)
 #include <algorithm>
 
 #include "dispatch.hpp"
@@ -48,20 +47,17 @@ __device__ __forceinline__ int entry_of(const MuonTable &t, int b) {
     return __builtin_amdgcn_readfirstlane(__popcll(__ballot(before)) - 1);
 }
 
-// One matrix in the workspace. X, A and P lie in panels of 64 bytes a row, all rows of a panel one after the other, so
-// that a tile's share of a panel is contiguous: an operand whose hi and lo parts are both multiplied has 16 columns a
-// panel, [16 hi | 16 lo]; one of which only the hi parts are has 32 columns a panel, and its lo parts a plane of their
-// own behind the first. A is of the first kind, X and P are what the call's products need.
+// One matrix in the workspace. X, A and P lie in panels of 16 columns, 64 bytes a row [16 hi | 16 lo], all rows of a
+// panel one after the other, so that a tile's share of a panel is contiguous.
 struct Planes {
     _Float16 *x0, *x1, *a, *p;
     double *part;
     size_t xs, as; // elements of X, of A
 };
-template<bool PAIRS>
-__device__ __forceinline__ size_t panel_at(int rows, int r, int c) { // of the hi part
-    return PAIRS ? (static_cast<size_t>(c >> 4) * rows + r) * 32 + (c & 15)
-                 : (static_cast<size_t>(c >> 5) * rows + r) * 32 + (c & 31);
+__device__ __forceinline__ size_t panel_at(int rows, int r, int c) { // of the hi part; the lo part is kLo further
+    return (static_cast<size_t>(c >> 4) * rows + r) * 32 + (c & 15);
 }
+constexpr int kLo = 16;
 __device__ __forceinline__ Planes planes_of(uint8_t *ws, const MuonEntry &e, int which) {
     Planes q;
     q.xs = static_cast<size_t>(e.mp) * e.np;
@@ -190,7 +186,7 @@ __global__ __launch_bounds__(256) void k_muon_momentum(MuonTable t, MuonParams p
 // X_0 = U scale / max(||U||, eps) in two fp16 parts, 64 x 64 tiles, by way of LDS: it is read along the rows of U and
 // written in the order of the panels, and a tall U is transposed between. Memory bound: 59 M fp32 elements 143 us,
 // 5.0 TB/s (190 us with 16 columns of one row per thread and no LDS).
-template<DType G, bool PAIRS>
+template<DType G>
 __global__ __launch_bounds__(256) void k_muon_start(MuonTable t, MuonParams p) {
     using S = typename Elem<G>::S;
     __shared__ float tile[64][65];
@@ -243,14 +239,14 @@ __global__ __launch_bounds__(256) void k_muon_start(MuonTable t, MuonParams p) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const int r = (threadIdx.x >> 2) & 63, piece = threadIdx.x & 3;
-        const bool low = PAIRS ? piece & 2 : k & 2;
-        const int x = PAIRS ? 16 * k + 8 * (piece & 1) : 32 * (k & 1) + 8 * piece;
+        const bool low = piece & 2;
+        const int x = 16 * k + 8 * (piece & 1);
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = tile[r][x + j];
         half8 hi, lo;
         split_fp16<8>(v, hi, lo);
-        _Float16 *to = q.x0 + panel_at<PAIRS>(e.mp, m0 + r, n0 + x) + (low ? PAIRS ? 16 : q.xs : 0);
+        _Float16 *to = q.x0 + panel_at(e.mp, m0 + r, n0 + x) + (low ? kLo : 0);
         *reinterpret_cast<half8 *>(to) = low ? lo : hi;
     }
 }
@@ -335,19 +331,17 @@ __device__ __forceinline__ int place_of_block() {
 // One product stage. A workgroup computes BM x BN of it. The M side's rows (of X, A or P) lie along the sum, and so do
 // the N side's of kGram and kPoly, which multiply by a transpose; kApply's and kFinal's N side is X itself, whose
 // fragments are transposed on their way out of LDS. Both sides travel straight to LDS, a panel of the sum at a time.
-// SPLIT: three products of the parts. PAIRS: X and P lie in pairs. The MFMA's first operand is the N side: a lane then
-// holds 4 neighbouring columns of one row. WV waves share a tile, two along m. KG groups of them take the panels in turn
-// and add their sums up at the end: with few tiles this fills the CUs. Of ST panels in a group's part of LDS one is
-// multiplied, the others are on their way.
+// The MFMA's first operand is the N side: a lane then holds 4 neighbouring columns of one row. WV waves share a tile, two
+// along m. KG groups of them take the panels in turn and add their sums up at the end: with few tiles this fills the
+// CUs. Of ST panels in a group's part of LDS one is multiplied, the others are on their way.
 //
 // What bounds it, 2 x 4096 x 4096: the matrix cores under the card's power limit. P X with three products runs at 1230
-// TFLOP/s issued (670 us), where the library's fp16 product of 8192^3 reaches 1170; with one product 905
-// (304 us). 12 x 768 x 768, 10 to 15 GFLOP a stage: 18 to 27 us, of which 9 do not depend on the length of the sum, the
+// TFLOP/s issued (670 us), where the library's fp16 product of 8192^3 reaches 1170. 12 x 768 x 768, 10 to 15 GFLOP a stage: 18 to 27 us, of which 9 do not depend on the length of the sum, the
 // start of a launch and the results on their way to memory behind it (14 to 28 MB: without the stores 12 to 25 us).
-template<int KIND, int BM, int BN, int WV, int KG, int ST, bool SPLIT, bool PAIRS, DType W>
+template<int KIND, int BM, int BN, int WV, int KG, int ST, DType W>
 __global__ __launch_bounds__(64 * WV * KG, KG == 1 ? 2 : 4) void k_muon_product(MuonTable t, MuonStage st) {
     constexpr int WM = BM / 2, WN = BN / (WV / 2), MT = WM / 32, NT = WN / 32;
-    constexpr int BK = SPLIT ? 16 : 32; // columns of a panel, the step along the sum
+    constexpr int BK = 16; // columns of a panel, the step along the sum
     constexpr bool NN = KIND == kApply || KIND == kFinal;
     constexpr bool AHEAD = MT * NT <= 4; // registers for two tiles' fragments
     constexpr int kTile = (BM + BN) * 64;
@@ -398,12 +392,9 @@ __global__ __launch_bounds__(64 * WV * KG, KG == 1 ? 2 : 4) void k_muon_product(
 #pragma unroll
     for (int k = 0; k < NI; ++k) {
         if constexpr (NN) { // BK rows of BN / BK panels
-            const int j = wave * NI + k, panels = e.np / BK;
-            const int pn = n0 / BK + j / (BK / 16);
-            np[k] = ns +
-                    (static_cast<size_t>(pn < panels ? pn : panels - 1) * rows + group * BK + j % (BK / 16) * 16 + lrow) *
-                        32 +
-                    (lpiece ^ (SPLIT ? (j & 1) << 1 : 0)) * 8;
+            const int j = wave * NI + k, panels = e.np / BK, pn = n0 / BK + j;
+            np[k] = ns + (static_cast<size_t>(pn < panels ? pn : panels - 1) * rows + group * BK + lrow) * 32 +
+                    (lpiece ^ ((j & 1) << 1)) * 8;
         } else {
             const int r = n0 + (wave * NI + k) * 16 + lrow;
             np[k] = ns + (static_cast<size_t>(group) * rows + (r < rows ? r : rows - 1)) * 32 + lpiece * 8;
@@ -434,15 +425,12 @@ __global__ __launch_bounds__(64 * WV * KG, KG == 1 ? 2 : 4) void k_muon_product(
         for (int z = 0; z < 2; ++z)
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                const int r = 8 * half + 4 * z + (l16 >> 2) + (SPLIT ? 0 : 16 * s);
-                const int piece = (SPLIT ? 2 * s : 2 * cb) + ((l16 & 3) >> 1);
-                const int panel = SPLIT ? wn / 16 + cb : wn / 32;
-                tr[z][s] = panel * (BK * 64) + r * 64 + ((piece ^ swizzle(r, SPLIT ? cb : 0)) << 4) + (l16 & 1) * 8;
+                const int r = 8 * half + 4 * z + (l16 >> 2);
+                const int piece = 2 * s + ((l16 & 3) >> 1), panel = wn / 16 + cb;
+                tr[z][s] = panel * (BK * 64) + r * 64 + ((piece ^ swizzle(r, cb)) << 4) + (l16 & 1) * 8;
             }
     }
-    constexpr bool kInPairs = NN ? PAIRS : true;  // layout of what the epilogue reads (X, or A)
-    const size_t in_lo = kInPairs ? 16 : q.xs;
-    const _Float16 *in = NN ? x : q.a;
+    const _Float16 *in = NN ? x : q.a; // what the epilogue reads
     const int nmax = NN ? e.np : rows;
     constexpr int LR = WN / 8, O = 32 / (64 / LR); // lanes of a row, and pieces of a slice of 32 rows of the results
     const auto mine_of = [&](int o) { return KG == 1 || o % KG == group; }; // pieces are shared out over the groups
@@ -451,9 +439,9 @@ __global__ __launch_bounds__(64 * WV * KG, KG == 1 ? 2 : 4) void k_muon_product(
         for (int o = 0; o < O; ++o) {
             const int m = m0 + wm + u * 32 + o * (64 / LR) + lane / LR, n = n0 + wn + lane % LR * 8;
             if (mine_of(o) && m < rows && n < nmax) {
-                const size_t at = panel_at<kInPairs>(rows, m, n);
+                const size_t at = panel_at(rows, m, n);
                 ih[o] = *reinterpret_cast<const half8 *>(in + at);
-                il[o] = *reinterpret_cast<const half8 *>(in + at + in_lo);
+                il[o] = *reinterpret_cast<const half8 *>(in + at + kLo);
             }
         }
     };
@@ -466,7 +454,7 @@ __global__ __launch_bounds__(64 * WV * KG, KG == 1 ? 2 : 4) void k_muon_product(
     float16v acc[NT][MT] = {};
     const int panels = K / BK, rounds = (panels + KG - 1) / KG, steps = (panels - group + KG - 1) / KG; // this group's
     const auto read = [&](int buf, half8 (&mf)[MT][2], half8 (&nf)[NT][2]) {
-        // two pieces of 16 of the sum: hi and lo of one, or both of 32
+        // [0]: the hi parts of 16 of the sum, [1]: the lo parts
         const uint8_t *ml = mine + buf * kTile, *nl = ml + BM * 64;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -478,7 +466,7 @@ __global__ __launch_bounds__(64 * WV * KG, KG == 1 ? 2 : 4) void k_muon_product(
                 for (int y = 0; y < NT; ++y) nf[y][s] = *reinterpret_cast<const half8 *>(nl + (wn + y * 32) * 64 + at);
             }
         }
-        if constexpr (NN) read_transposed<NT, 32 / BK * BK * 64>(nl, tr, nf);
+        if constexpr (NN) read_transposed<NT, 32 * 64>(nl, tr, nf);
     };
     const auto multiply = [&](const half8 (&mf)[MT][2], const half8 (&nf)[NT][2]) {
         const auto mul = [&](int sn, int sm) {
@@ -489,12 +477,8 @@ __global__ __launch_bounds__(64 * WV * KG, KG == 1 ? 2 : 4) void k_muon_product(
                     acc[y][u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(nf[y][sn], mf[u][sm], acc[y][u], 0, 0, 0);
         };
         mul(0, 0);
-        if constexpr (SPLIT) {
-            mul(0, 1);
-            mul(1, 0);
-        } else {
-            mul(1, 1);
-        }
+        mul(0, 1);
+        mul(1, 0);
     };
     if constexpr (AHEAD) {
         // the next tile's fragments are read while this one's are multiplied
@@ -564,10 +548,7 @@ __global__ __launch_bounds__(64 * WV * KG, KG == 1 ? 2 : 4) void k_muon_product(
         v *= 1.0f / kMuonScaleX;
         return static_cast<WS>(step ? static_cast<float>(old) * st.decay - alpha * v : v);
     };
-    constexpr bool kOutPairs = KIND == kGram || PAIRS; // layout of what is written (A, P or X)
-    const size_t out_lo = kOutPairs ? 16 : q.xs;
     _Float16 *out = KIND == kGram ? q.a : KIND == kPoly ? q.p : st.cur ? q.x0 : q.x1;
-    const bool lows = KIND != kPoly || PAIRS; // P's lo parts are only there to be multiplied
 #pragma unroll
     for (int u = 0; u < MT; ++u) {
         const int mb = m0 + wm + u * 32;
@@ -623,9 +604,9 @@ __global__ __launch_bounds__(64 * WV * KG, KG == 1 ? 2 : 4) void k_muon_product(
             if constexpr (KIND != kFinal) {
                 half8 oh, ol;
                 split_fp16<8>(v, oh, ol);
-                const size_t at = panel_at<kOutPairs>(rows, m, n);
+                const size_t at = panel_at(rows, m, n);
                 *reinterpret_cast<half8 *>(out + at) = oh;
-                if (lows) *reinterpret_cast<half8 *>(out + at + out_lo) = ol;
+                *reinterpret_cast<half8 *>(out + at + kLo) = ol;
             }
             if (KIND != kApply) { // read again, along the columns or by other lanes
                 *reinterpret_cast<float4 *>(slice + r * kPitch + c) = *reinterpret_cast<float4 *>(v);
@@ -646,9 +627,9 @@ __global__ __launch_bounds__(64 * WV * KG, KG == 1 ? 2 : 4) void k_muon_product(
                     for (int k = 0; k < 8; ++k) v[k] = slice[(r + k) * kPitch + c];
                     half8 oh, ol;
                     split_fp16<8>(v, oh, ol);
-                    const size_t at = panel_at<kOutPairs>(rows, n, mb + r);
+                    const size_t at = panel_at(rows, n, mb + r);
                     *reinterpret_cast<half8 *>(out + at) = oh;
-                    if (lows) *reinterpret_cast<half8 *>(out + at + out_lo) = ol;
+                    *reinterpret_cast<half8 *>(out + at + kLo) = ol;
                 }
             }
         }
@@ -1015,15 +996,15 @@ int64_t product_tiles(int kind, const MuonEntry &e) {
     return tm * ((e.mp + BN - 1) / BN) - BM / BN * (tm * (tm - 1) / 2);
 }
 
-template<int KIND, int BM, int BN, int WV, int KG, int ST, bool SPLIT, bool PAIRS, DType W>
+template<int KIND, int BM, int BN, int WV, int KG, int ST, DType W>
 bool launch_product(MuonTable &t, const MuonStage &st, hipStream_t s) {
     const int64_t n = layout(t, [](const MuonEntry &e) { return product_tiles<BM, BN>(KIND, e); });
     if (n > INT32_MAX) return false;
     const dim3 grid(static_cast<unsigned>(n));
-    return launch_ok([&] { k_muon_product<KIND, BM, BN, WV, KG, ST, SPLIT, PAIRS, W><<<grid, 64 * WV * KG, 0, s>>>(t, st); });
+    return launch_ok([&] { k_muon_product<KIND, BM, BN, WV, KG, ST, W><<<grid, 64 * WV * KG, 0, s>>>(t, st); });
 }
 
-template<int KIND, bool SPLIT, bool PAIRS, DType W = DType::F32>
+template<int KIND, DType W = DType::F32>
 bool launch_stage(MuonTable &t, const MuonStage &st, hipStream_t s) {
     // Tiles by an estimate of a launch's time: some us, and for each panel of the sum the time of a tile times the tiles
     // of a CU, between the average and the fullest CU's (where two fit a CU an odd one out takes a quarter longer, where
@@ -1038,7 +1019,7 @@ bool launch_stage(MuonTable &t, const MuonStage &st, hipStream_t s) {
     double panels = 0.0, all = 0.0;
     for (int i = 0; i < t.n; ++i) {
         const double tiles = static_cast<double>(t.e[i].count) * product_tiles<64, 64>(KIND, t.e[i]);
-        panels += tiles * (KIND == kGram ? t.e[i].np : t.e[i].mp) / (SPLIT ? 16 : 32);
+        panels += tiles * (KIND == kGram ? t.e[i].np : t.e[i].mp) / 16;
         all += tiles;
     }
     panels /= all;
@@ -1058,12 +1039,12 @@ bool launch_stage(MuonTable &t, const MuonStage &st, hipStream_t s) {
         cost([](const MuonEntry &e) { return product_tiles<64, 32>(KIND, e); }, 4.2, 0.084),
     };
     switch (std::min_element(est, est + 6) - est) {
-        case 0: return launch_product<KIND, 256, 128, 4, 1, 3, SPLIT, PAIRS, W>(t, st, s);
-        case 1: return launch_product<KIND, 128, 128, 4, 1, 3, SPLIT, PAIRS, W>(t, st, s);
-        case 2: return launch_product<KIND, 128, 64, 4, 1, 3, SPLIT, PAIRS, W>(t, st, s);
-        case 3: return launch_product<KIND, 64, 64, 4, 2, 3, SPLIT, PAIRS, W>(t, st, s);
-        case 4: return launch_product<KIND, 64, 64, 4, 4, 3, SPLIT, PAIRS, W>(t, st, s);
-        default: return launch_product<KIND, 64, 32, 2, 4, 3, SPLIT, PAIRS, W>(t, st, s);
+        case 0: return launch_product<KIND, 256, 128, 4, 1, 3, W>(t, st, s);
+        case 1: return launch_product<KIND, 128, 128, 4, 1, 3, W>(t, st, s);
+        case 2: return launch_product<KIND, 128, 64, 4, 1, 3, W>(t, st, s);
+        case 3: return launch_product<KIND, 64, 64, 4, 2, 3, W>(t, st, s);
+        case 4: return launch_product<KIND, 64, 64, 4, 4, 3, W>(t, st, s);
+        default: return launch_product<KIND, 64, 32, 2, 4, 3, W>(t, st, s);
     }
 }
 
@@ -1093,13 +1074,6 @@ bool launch_muon(const MuonEntry *entries, int n, DType gt, DType wt, const Muon
         to.e[to.n++] = entries[i];
         if (&to == &narrow) np = np > entries[i].np ? np : entries[i].np;
     }
-    // Three products everywhere: where the result has more bits than one product, and for small matrices, whose sums are
-    // too short to average the roundings of one product out (sides below 200: up to 1.46 times the error of the bf16
-    // result's own rounding, against 1.00; 1.1 to 1.36 from 320 to 2048). In us, one product / three: 12 x 256 x 256
-    // 92 / 105, 12 x 256 x 1024 124 / 153, 48 x 256 x 1024 265 / 364; above, 12 x 768 x 768 348 / 502.
-    int largest = 0;
-    for (int i = 0; i < t.n; ++i) largest = std::max(largest, t.e[i].mp);
-    const bool pairs = wt != DType::BF16 || largest <= 256;
     const auto with_grad = [&](auto &&f) {
         switch (gt) {
             case DType::F32: return f(std::integral_constant<DType, DType::F32>{});
@@ -1121,12 +1095,7 @@ bool launch_muon(const MuonEntry *entries, int n, DType gt, DType wt, const Muon
             return false;
         blocks = layout(t, [](const MuonEntry &e) { return static_cast<int64_t>(e.mp / 64) * (e.np / 64); });
         if (blocks > INT32_MAX) return false;
-        return launch_ok([&] {
-            if (pairs)
-                k_muon_start<G, true><<<dim3(static_cast<unsigned>(blocks)), 256, 0, s>>>(t, p);
-            else
-                k_muon_start<G, false><<<dim3(static_cast<unsigned>(blocks)), 256, 0, s>>>(t, p);
-        });
+        return launch_ok([&] { k_muon_start<G><<<dim3(static_cast<unsigned>(blocks)), 256, 0, s>>>(t, p); });
     });
     if (!started) return false;
     if (t.n == 0) return true;
@@ -1136,18 +1105,16 @@ bool launch_muon(const MuonEntry *entries, int n, DType gt, DType wt, const Muon
     std::stable_sort(by_n.e, by_n.e + by_n.n, [](const MuonEntry &x, const MuonEntry &y) { return x.np > y.np; });
     for (int k = 0; k < p.steps; ++k) {
         const MuonStage st{k & 1, p.a, p.b, p.c, p.decay};
-        bool ok = pairs ? launch_stage<kGram, true, true>(by_n, st, s) && launch_stage<kPoly, true, true>(t, st, s)
-                        : launch_stage<kGram, false, false>(by_n, st, s) && launch_stage<kPoly, true, false>(t, st, s);
+        bool ok = launch_stage<kGram>(by_n, st, s) && launch_stage<kPoly>(t, st, s);
         if (!ok) return false;
         if (k + 1 < p.steps)
-            ok = pairs ? launch_stage<kApply, true, true>(t, st, s) : launch_stage<kApply, false, false>(t, st, s);
+            ok = launch_stage<kApply>(t, st, s);
         else if (wt == DType::F32)
-            ok = launch_stage<kFinal, true, true, DType::F32>(t, st, s);
+            ok = launch_stage<kFinal, DType::F32>(t, st, s);
         else if (wt == DType::F16)
-            ok = launch_stage<kFinal, true, true, DType::F16>(t, st, s);
+            ok = launch_stage<kFinal, DType::F16>(t, st, s);
         else
-            ok = pairs ? launch_stage<kFinal, true, true, DType::BF16>(t, st, s)
-                       : launch_stage<kFinal, false, false, DType::BF16>(t, st, s);
+            ok = launch_stage<kFinal, DType::BF16>(t, st, s);
         if (!ok) return false;
     }
     return true;

@@ -85,9 +85,8 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence[flo
     """The orthogonal factor of each matrix of ``x`` ([..., m, n], fp32 / bf16 / fp16), by ``steps`` Newton-Schulz
     steps from ``x / max(||x||_F, eps)``; singular values end near 1, in about [0.7, 1.2] with the default coefficients.
 
-    Not differentiable. The norm is summed in 64 bits; an fp32 or fp16 result has the error of fp32 products, a bf16
-    result one rounding more than bf16's own. A zero matrix gives zero, one with a NaN or an infinity gives NaN.
-    Non-contiguous input is copied. ``out`` (contiguous, of x's shape and type) may be ``x`` itself.
+    Not differentiable. The norm is summed in 64 bits; a result has the error of fp32 products and one rounding to its
+    type. A zero matrix gives zero, one with a NaN or an infinity gives NaN. Non-contiguous input is copied. ``out`` (contiguous, of x's shape and type) may be ``x`` itself.
     """
     coefficients, steps = tuple(map(float, coefficients)), index(steps)
     _check_coefficients(coefficients, steps)

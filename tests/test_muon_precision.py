@@ -1,0 +1,68 @@
+"""Every result has the error of products of 22-bit operands, also a bf16 one, whatever else the call holds.
+
+The model of tests/test_muon.py with pairs everywhere (`deviation(x, False)`): three times its deviation, and the rounding
+of the result's type.
+"""
+import pytest
+import torch
+
+from pccl_amd.ops import muon_step, orthogonalize
+from test_muon import deviation, exact, gradient
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+@pytest.fixture(params=DEVICES)
+def device(request):
+    if request.param == "cuda":
+        request.getfixturevalue("hip")
+    return torch.device(request.param)
+
+
+def check_pairs(x, got):
+    want = exact(x)
+    allowed = 3 * deviation(x, False) + want.abs() * (torch.finfo(got.dtype).eps / 2 * 1.01)
+    off = (got.double() - want).abs() - allowed
+    assert bool((off <= torch.finfo(got.dtype).smallest_normal).all()), f"off by {float(off.max())} more than allowed"
+
+
+@pytest.mark.parametrize("shape", [(65, 300), (3, 256, 192), (300, 500), (400, 320)])
+def test_bf16_of_few_rows(device, shape):
+    x = gradient(shape, 21, device, BF16)
+    check_pairs(x, orthogonalize(x))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(320, 1000), (12, 768, 768), (1030, 2050), (2050, 1030), (1, 4096, 1100)])
+def test_bf16_of_many_rows(hip, shape):
+    """Enough rows for every tile that bf16 matrices take."""
+    x = gradient(shape, 22, hip, BF16)
+    check_pairs(x, orthogonalize(x))
+
+
+@pytest.mark.gpu
+def test_bf16_beside_a_larger_matrix(hip):
+    """A small matrix is as exact next to a large one as it is alone, in either order."""
+    shapes = [(17, 900), (100, 300), (1000, 1500), (250, 260), (64, 512), (700, 520)]
+    for order in (shapes, shapes[::-1]):
+        grads = [gradient(s, 30 + s[0], hip, BF16) for s in order]
+        params = [torch.zeros_like(g) for g in grads]
+        muon_step(params, grads, [torch.zeros(s, device=hip) for s in order], lr=-1.0, weight_decay=0.0, momentum=0.0,
+                  adjust_lr="none")
+        for p, g in zip(params, grads):
+            check_pairs(g, p)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wtype,gtype", [(F16, F16), (F32, BF16), (BF16, F32), (F16, F32), (F32, F16)])
+def test_types_at_staged_sizes(hip, wtype, gtype):
+    """Parameters and gradients of every type, at sizes of several tiles and more entries than a launch takes."""
+    shapes = [(1100, 700), (520, 2050), (300, 400), (64, 900), (1030, 1030), (130, 70)] + [(70 + i, 140) for i in range(50)]
+    grads = [gradient(s, 40 + i, hip, gtype) for i, s in enumerate(shapes)]
+    params = [torch.zeros(s, device=hip, dtype=wtype) for s in shapes]
+    moms = [torch.zeros(s, device=hip) for s in shapes]
+    muon_step(params, grads, moms, lr=-1.0, weight_decay=0.0, momentum=0.0, adjust_lr="none")
+    for p, g, b in zip(params, grads, moms):
+        assert torch.equal(b, g.float())
+        check_pairs(g, p)
