@@ -4,6 +4,7 @@ from __future__ import annotations
 from contextlib import nullcontext
 
 import torch
+from torch.autograd import forward_ad
 
 from .kernels import hip_device_count
 
@@ -14,6 +15,14 @@ _HERE = nullcontext()
 def require_hip() -> None:
     if hip_device_count() == 0:
         raise RuntimeError("pccl-amd HIP backend (libpccl_hip.so) is not loaded but a GPU tensor was passed")
+
+
+def refuse_tangents(what: str, *tensors: torch.Tensor) -> None:
+    """The kernels have no forward-mode derivative, and a dual tensor's tangent would be dropped without a word."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # outside of every dual_level()
+        return
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what}: no forward-mode derivative of the HIP kernels, got a tensor with a tangent")
 
 
 def refuse_inference(what: str, *written: torch.Tensor) -> None:

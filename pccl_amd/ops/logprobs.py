@@ -12,7 +12,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from .._native import C
-from ._launch import on_device, require_hip, stream_of
+from ._launch import on_device, refuse_tangents, require_hip, stream_of
 from .kernels import WIRE_DTYPE, _check
 
 MAX_TOP_LOGPROBS = 64
@@ -175,9 +175,10 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top_k: int = 
     * a row whose every logit is ``-inf`` has entropy 0, log probabilities ``-inf`` and gradient 0;
     * a row with a NaN or ``+inf`` has NaN results and gradients.
 
-    ``logprob``, ``entropy`` and ``top_logprob`` are differentiable (once) with respect to ``logits``; the call and its
-    backward only queue kernels, so both may be captured into a graph. (Before a backward pass is captured, drop the
-    results of eager calls on the same leaves: torch ends the process when their graph is still alive.)
+    ``logprob``, ``entropy`` and ``top_logprob`` are differentiable with respect to ``logits``, once and in backward
+    mode (logits on a GPU with a forward-mode tangent are refused). The call and its backward only queue kernels, so both
+    may be captured into a graph. (Before a backward pass is captured, drop the results of eager calls on the same
+    leaves: torch ends the process when their graph is still alive.)
     """
     top_k, ignore_index = index(top_k), index(ignore_index)
     if logits.dim() < 1 or logits.shape[-1] < 1:
@@ -199,6 +200,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top_k: int = 
         raise ValueError("token_logprobs: at most 2^31 - 1 rows and tokens of vocabulary")
     if logits.device.type == "cuda":
         require_hip()
+        refuse_tangents("token_logprobs", logits)
     elif logits.device.type != "cpu":
         raise ValueError(f"token_logprobs: no kernel for device {logits.device}")
     if logits.requires_grad and torch.is_grad_enabled():

@@ -17,7 +17,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from .._native import C
-from ._launch import on_device, refuse_inference, require_hip, stream_of
+from ._launch import on_device, refuse_inference, refuse_tangents, require_hip, stream_of
 from .kernels import WIRE_DTYPE, _check
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
@@ -85,8 +85,8 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence[flo
     """The orthogonal factor of each matrix of ``x`` ([..., m, n], fp32 / bf16 / fp16), by ``steps`` Newton-Schulz
     steps from ``x / max(||x||_F, eps)``; singular values end near 1, in about [0.7, 1.2] with the default coefficients.
 
-    Not differentiable. The norm is summed in 64 bits; a result has the error of fp32 products and one rounding to its
-    type. A zero matrix gives zero, one with a NaN or an infinity gives NaN. Non-contiguous input is copied. ``out`` (contiguous, of x's shape and type) may be ``x`` itself.
+    Not differentiable (on a GPU a tensor with a forward-mode tangent is refused). The norm is summed in 64 bits; a result
+    has the error of fp32 products and one rounding to its type. A zero matrix gives zero, one with a NaN or an infinity gives NaN. Non-contiguous input is copied. ``out`` (contiguous, of x's shape and type) may be ``x`` itself.
     """
     coefficients, steps = tuple(map(float, coefficients)), index(steps)
     _check_coefficients(coefficients, steps)
@@ -111,6 +111,7 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence[flo
         return out.copy_(_host_orthogonalize(x, steps, coefficients, eps))
     if x.device.type != "cuda":
         raise ValueError(f"orthogonalize: no kernel for device {x.device}")
+    refuse_tangents("orthogonalize", x, out)
     m, n = x.shape[-2:]
     x = x.contiguous()
     _queue((x.numel() // (m * n), m, n), (x.data_ptr(),), x.dtype, (out.data_ptr(),), x.dtype, None, None, 1.0, 0.0, 0,
@@ -197,6 +198,7 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     alpha = [factors[e[:2]] for e in work]
     decay = 1.0 - lr * weight_decay
     if device.type == "cuda":
+        refuse_tangents("muon_step", *(t for e in work for t in e[2:]))
         _queue([v for e in work for v in (1, e[0], e[1])], [e[3].data_ptr() for e in work], gtype,
                [e[2].data_ptr() for e in work], wtype, [e[4].data_ptr() for e in work], alpha, decay, momentum,
                int(nesterov), steps, coefficients, eps, device, "muon_step")
