@@ -344,6 +344,7 @@ __global__ __launch_bounds__(64 * WV * KG, KG == 1 ? 2 : 4) void k_muon_product(
     constexpr int BK = 16; // columns of a panel, the step along the sum
     constexpr bool NN = KIND == kApply || KIND == kFinal;
     constexpr bool AHEAD = MT * NT <= 4; // registers for two tiles' fragments
+    static_assert(AHEAD || KG == 1, "the other loop has no round without a panel");
     constexpr int kTile = (BM + BN) * 64;
     constexpr int kSlice = 32 * (WN + 4) * 4; // 32 rows of a wave's results, padded against bank conflicts
     constexpr int kLds = KG * (ST * kTile > WV * kSlice ? ST * kTile : WV * kSlice);
@@ -509,12 +510,11 @@ __global__ __launch_bounds__(64 * WV * KG, KG == 1 ? 2 : 4) void k_muon_product(
 #pragma unroll
         for (int k = 0; k < ST - 1; ++k)
             if (k < steps) fetch(k);
-        for (int k = 0, buf = 0, to = ST - 1; k < rounds; ++k) {
+        for (int k = 0, buf = 0, to = ST - 1; k < steps; ++k) {
             const int later = steps - 1 - k; // tiles behind this one
             wait_tiles<MI + NI, ST - 1>(later < ST - 2 ? (later > 0 ? later : 0) : ST - 2);
             __builtin_amdgcn_s_barrier(); // tile k has landed for every wave, and all are done with tile k - 1
             asm volatile("" ::: "memory");
-            if (KG > 1 && k >= steps) break; // the last round, without a panel for this group
             half8 mf[MT][2], nf[NT][2];
             read(buf, mf, nf);
             if (k + ST - 1 < steps) fetch(to); // over tile k - 1

@@ -6,7 +6,7 @@
 //
 // Three matrix products a step, all on the matrix cores with 16-bit operands and 32-bit sums. An fp32 value v is held
 // as two fp16 numbers v * scale = hi + lo (22 bits); a product of two such values is hi hi + hi lo + lo hi. The scales
-// are fixed powers of two (below): X stays below kMuonMaxNorm in the 2-norm, which the host checks for the
+// are fixed powers of two (below): X stays below 4 and P below 12 in the 2-norm, which the host checks for the
 // coefficients of the call, so every entry of X, A and P is in range and its lo part far above fp16's smallest step.
 //
 // The Muon step wraps it:  B += (1 - mu)(G - B);  U = G + mu (B - G) (Nesterov) or B;  O = orthogonalised U;
