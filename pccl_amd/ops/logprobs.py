@@ -171,7 +171,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top_k: int = 
 
     * targets equal to ``ignore_index`` have log probability 0 and no gradient through it;
     * a target outside the vocabulary has log probability NaN, and NaN gradients (checking it would wait for the GPU);
-    * ``-inf`` logits are masked tokens: probability 0, no share in the entropy, gradient 0;
+    * ``-inf`` logits are masked tokens: probability 0, no share in the entropy, gradient 0; only a masked
+      target or alternative, of log probability ``-inf``, gets its upstream gradient (times 1 - p = 1);
     * a row whose every logit is ``-inf`` has entropy 0, log probabilities ``-inf`` and gradient 0;
     * a row with a NaN or ``+inf`` has NaN results and gradients.
 

@@ -436,3 +436,29 @@ def test_every_element_counts_once(device, dtype, vocab, top_k):
     want = -p
     want.scatter_add_(1, targets[:, None], torch.ones(n, 1, dtype=torch.float64))
     close(d, want, want.abs() * torch.finfo(dtype).eps / 2 * 1.01 + 64 * U)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradient_of_masked_targets_and_alternatives(device, dtype):
+    """Their log probability is -inf; 1 - p = 1 of their upstream gradient reaches them, and nothing a masked token that
+    is neither."""
+    x = torch.full((3, 40), -math.inf, dtype=dtype, device=device)
+    x[:, :3] = torch.tensor([1.0, 2.0, 0.5], dtype=dtype, device=device)
+    t = torch.tensor([1, 7, 4], device=device)
+    leaf = x.requires_grad_()
+    r = token_logprobs(leaf, t, top_k=5)
+    assert r.top_index.tolist() == [[1, 0, 2, 3, 4]] * 3
+    assert r.logprob.isneginf().tolist() == [False, True, True] and bool(r.top_logprob[:, 3:].isneginf().all())
+    g_lp, g_top = torch.tensor([1.0, 2.0, 4.0], device=device), torch.arange(1.0, 6.0, device=device).repeat(3, 1)
+    d, = torch.autograd.grad([r.logprob, r.top_logprob], leaf, [g_lp, g_top])
+    want = torch.zeros(3, 40)
+    want[:, 3:5] += torch.tensor([4.0, 5.0])  # exact in every type
+    want[1, 7] += 2.0
+    want[2, 4] += 4.0
+    assert torch.equal(d[:, 3:].cpu().float(), want[:, 3:])
+    # p is off by at most 64 u; the upstream gradients add up to at most 20
+    p = torch.softmax(x[:, :3].detach().cpu().double(), dim=1)
+    at = torch.tensor([[2.0, 1.0, 3.0]]).repeat(3, 1).double()  # alternatives' own
+    at[0, 1] += 1.0
+    close(d[:, :3], at - p * (15.0 + g_lp.cpu()[:, None]),
+          64 * U * 20 + torch.finfo(dtype).eps / 2 * (at - p * (15.0 + g_lp.cpu()[:, None])).abs() * 1.01)
