@@ -5,6 +5,10 @@ Muon replaces the momentum update U of a weight matrix by its orthogonal factor,
 optimiser (:class:`pccl_amd.parallel.Muon`). GPU tensors run the HIP kernels (csrc/hip/hip_muon.hip) on the current
 stream without synchronising: every matrix of a call, whatever its shape, goes through each stage in one launch. CPU
 tensors run plain torch operations.
+
+A call on the GPU takes a workspace from torch's allocator for its own duration: 8 bytes for each element of X and of
+X X^T (sides padded to 64) of every matrix that does not fit in LDS, at most 4 GiB (further matrices take turns in it),
+or what one larger matrix needs (20 GiB for 30000 x 60000).
 """
 from __future__ import annotations
 
@@ -87,6 +91,7 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence[flo
 
     Not differentiable (on a GPU a tensor with a forward-mode tangent is refused). The norm is summed in 64 bits; a result
     has the error of fp32 products and one rounding to its type. A zero matrix gives zero, one with a NaN or an infinity gives NaN. Non-contiguous input is copied. ``out`` (contiguous, of x's shape and type) may be ``x`` itself.
+    Equal calls give equal bits; a matrix in another stack may differ in its last bits.
     """
     coefficients, steps = tuple(map(float, coefficients)), index(steps)
     _check_coefficients(coefficients, steps)
@@ -157,7 +162,8 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     ``params``: contiguous 2-D, one type of fp32 / bf16 / fp16; ``grads``: of their shapes, one type of the same three,
     non-contiguous ones are copied; ``momentum_buffers``: contiguous fp32. All on one device, none of them sharing
     memory with another (a parameter listed twice is refused; a gradient may serve several parameters). Equal calls give
-    equal bits on every peer. The call may be captured into a graph, which then keeps its learning rate.
+    equal bits on every peer; which matrices share a call decides the order of their sums, so that the same matrix in
+    another call may differ in its last bits. The call may be captured into a graph, which then keeps its learning rate.
     """
     coefficients, steps = tuple(map(float, coefficients)), index(steps)
     check_muon("muon_step", lr, weight_decay, momentum, steps, coefficients, eps, adjust_lr)
