@@ -335,9 +335,10 @@ __device__ __forceinline__ int place_of_block() {
 // along m. KG groups of them take the panels in turn and add their sums up at the end: with few tiles this fills the
 // CUs. Of ST panels in a group's part of LDS one is multiplied, the others are on their way.
 //
-// What bounds it, 2 x 4096 x 4096: the matrix cores under the card's power limit. P X with three products runs at 1230
-// TFLOP/s issued (670 us), where the library's fp16 product of 8192^3 reaches 1170. 12 x 768 x 768, 10 to 15 GFLOP a stage: 18 to 27 us, of which 9 do not depend on the length of the sum, the
-// start of a launch and the results on their way to memory behind it (14 to 28 MB: without the stores 12 to 25 us).
+// What bounds it, 2 x 4096 x 4096: P X the matrix cores under the card's power limit, 1180 TFLOP/s issued (700 us), where
+// the library's fp16 product of 8192^3 reaches 1200. X X^T and A A reach 950 (445 us): their 1056 tiles on and above the
+// diagonal are 4.1 a CU, and the fullest has 5. 12 x 768 x 768, 19 to 33 GFLOP issued a stage: 30 to 46 us, of which 8 to 9
+// do not depend on the length of the sum, the start of a launch and the results on their way to memory behind it.
 template<int KIND, int BM, int BN, int WV, int KG, int ST, DType W>
 __global__ __launch_bounds__(64 * WV * KG, KG == 1 ? 2 : 4) void k_muon_product(MuonTable t, MuonStage st) {
     constexpr int WM = BM / 2, WN = BN / (WV / 2), MT = WM / 32, NT = WN / 32;
