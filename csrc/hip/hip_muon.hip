@@ -52,7 +52,6 @@ __device__ __forceinline__ int entry_of(const MuonTable &t, int b) {
 struct Planes {
     _Float16 *x0, *x1, *a, *p;
     double *part;
-    size_t xs, as; // elements of X, of A
 };
 __device__ __forceinline__ size_t panel_at(int rows, int r, int c) { // of the hi part; the lo part is kLo further
     return (static_cast<size_t>(c >> 4) * rows + r) * 32 + (c & 15);
@@ -60,15 +59,14 @@ __device__ __forceinline__ size_t panel_at(int rows, int r, int c) { // of the h
 constexpr int kLo = 16;
 __device__ __forceinline__ Planes planes_of(uint8_t *ws, const MuonEntry &e, int which) {
     Planes q;
-    q.xs = static_cast<size_t>(e.mp) * e.np;
-    q.as = static_cast<size_t>(e.mp) * e.mp;
-    const size_t bytes = 2 * (4 * q.xs + 4 * q.as) + kMuonMaxPartials * sizeof(double);
+    const size_t xs = static_cast<size_t>(e.mp) * e.np, as = static_cast<size_t>(e.mp) * e.mp; // elements of X, of A
+    const size_t bytes = 2 * (4 * xs + 4 * as) + kMuonMaxPartials * sizeof(double);
     uint8_t *base = ws + e.off + bytes * which;
     q.x0 = reinterpret_cast<_Float16 *>(base);
-    q.x1 = q.x0 + 2 * q.xs;
-    q.a = q.x1 + 2 * q.xs;
-    q.p = q.a + 2 * q.as;
-    q.part = reinterpret_cast<double *>(q.p + 2 * q.as);
+    q.x1 = q.x0 + 2 * xs;
+    q.a = q.x1 + 2 * xs;
+    q.p = q.a + 2 * as;
+    q.part = reinterpret_cast<double *>(q.p + 2 * as);
     return q;
 }
 
