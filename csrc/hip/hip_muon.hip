@@ -674,11 +674,11 @@ __global__ __launch_bounds__(64 * WV * KG, KG == 1 ? 2 : 4) void k_muon_product(
 }
 
 // Everything for a matrix that fits in LDS, by one workgroup: X, and A / P in one place, in paired panels as above and
-// with three products throughout. A wave has whole 32 x 32 tiles of the products, so nothing is joined between waves,
+// with three products, up to 32 rows four for A and A A. A wave has whole 32 x 32 tiles of the products, so nothing is joined between waves,
 // and keeps its own entries of X and A in registers from product to product. Bound by LDS reads, products and barriers
-// in turn; us of a call of orthogonalize / the Muon step: 64 x 64 13 / 15 (4 waves; sharing each tile's sum between 2
-// or 4 waves 17 / 21), 64 x 256 26 / 29 (8 waves; 4, which read least, 36), 256 x 64 27 / 31, 128 x 128 38 / 41 (16
-// waves; 8 40 / 43). 1000 of 64 x 64 35 us. The 17 launches of the stages took 77 for 64 x 64.
+// in turn; us of a call of orthogonalize / the Muon step: 64 x 64 14 / 16 (4 waves; sharing each tile's sum between 2
+// or 4 waves 17 / 21), 64 x 256 28 / 31 (8 waves; 4, which read least, 36), 256 x 64 29 / 32, 128 x 128 39 / 42 (16
+// waves; 8 40 / 43). 1000 of 64 x 64 40 us. The 17 launches of the stages took 77 for 64 x 64.
 template<int MP, int NP, int NW, DType G, DType W>
 __global__ __launch_bounds__(64 * NW) void k_muon_small(MuonTable t, MuonParams p) {
     using S = typename Elem<G>::S;
@@ -847,8 +847,13 @@ __global__ __launch_bounds__(64 * NW) void k_muon_small(MuonTable t, MuonParams 
     const int ar = wave * RA % MB * 32, ac = wave * RA / MB * 32;
     const int xr = wave * RM % MB * 32, xc = wave * RM / MB * 32;
     const bool has_a = NA == NW || wave < NA, has_x = NP == MP || xc < np;
-    // this wave's tiles of `base` times its own transpose
-    const auto square = [&](const uint8_t *base, int panels, float16v (&out)[RA]) {
+    // This wave's tiles of `base` times its own transpose. hi lo + lo hi get a sum of their own (in one sum with hi hi they
+    // round it three times as often), and up to 32 rows lo lo is added too: so few rows leave nothing for these roundings to
+    // average out over. Error over that of the same steps in fp32, 64 x 64 0.88 -> 0.76 (14.0 -> 14.4 us), 64 x 256 1.0 -> 0.8
+    // (26.8 -> 27.9), 16 x 230 1.8 -> 1.3 (27.4 -> 29.7; without lo lo 1.45); 128 x 128 0.8 as it is, with no register free.
+    constexpr bool kApart = MP == 64;
+    const auto square_by = [&](auto four, const uint8_t *base, int panels, float16v (&out)[RA]) {
+        float16v low[kApart ? RA : 1] = {};
 #pragma unroll
         for (int k = 0; k < RA; ++k) out[k] = float16v{};
 #pragma unroll (MP == 128 ? 2 : 4)
@@ -857,9 +862,27 @@ __global__ __launch_bounds__(64 * NW) void k_muon_small(MuonTable t, MuonParams 
 #pragma unroll
             for (int k = 0; k < RA; ++k) {
                 const half8 m[2] = {frag(base, ar + 32 * k, s, 0), frag(base, ar + 32 * k, s, 1)};
-                out[k] = mul3(out[k], n, m);
+                if constexpr (kApart) {
+                    out[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(n[0], m[0], out[k], 0, 0, 0);
+                    low[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(n[0], m[1], low[k], 0, 0, 0);
+                    low[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(n[1], m[0], low[k], 0, 0, 0);
+                    if constexpr (decltype(four)::value)
+                        low[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(n[1], m[1], low[k], 0, 0, 0);
+                } else {
+                    out[k] = mul3(out[k], n, m);
+                }
             }
         }
+        if constexpr (kApart) {
+#pragma unroll
+            for (int k = 0; k < RA; ++k) out[k] += low[k];
+        }
+    };
+    const auto square = [&](const uint8_t *base, int panels, float16v (&out)[RA]) {
+        if (kApart && ms <= 32)
+            square_by(std::true_type{}, base, panels, out);
+        else
+            square_by(std::false_type{}, base, panels, out);
     };
 
     __syncthreads(); // X is written

@@ -66,3 +66,21 @@ def test_types_at_staged_sizes(hip, wtype, gtype):
     for p, g, b in zip(params, grads, moms):
         assert torch.equal(b, g.float())
         check_pairs(g, p)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(16, 16), (16, 230), (230, 16), (20, 100), (17, 40), (31, 256), (64, 64), (64, 256),
+                                   (128, 128), (70, 300), (16, 1000)])
+def test_fp32_of_small_matrices(hip, shape):
+    """Few rows leave little for roundings to average out over: root mean square errors of 32 matrices, at most half again
+    those of the same steps in fp32 products."""
+    x = torch.stack([gradient(shape, 200 + i, hip) for i in range(32)])
+    want = exact(x)
+    y = (x / x.double().square().sum((-2, -1), keepdim=True).sqrt()).float()
+    y = y.mT.contiguous() if shape[0] > shape[1] else y
+    for _ in range(5):
+        g = y @ y.mT.contiguous()
+        y = 3.4445 * y + (-4.7750 * g + 2.0315 * (g @ g)) @ y
+    y = y.mT if shape[0] > shape[1] else y
+    error = lambda t: float((t.double() - want).square().mean().sqrt())  # noqa: E731
+    assert error(orthogonalize(x)) <= 1.5 * error(y), (error(orthogonalize(x)), error(y))
