@@ -84,3 +84,35 @@ def test_fp32_of_small_matrices(hip, shape):
     y = y.mT if shape[0] > shape[1] else y
     error = lambda t: float((t.double() - want).square().mean().sqrt())  # noqa: E731
     assert error(orthogonalize(x)) <= 1.5 * error(y), (error(orthogonalize(x)), error(y))
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(hip):
+    """More than 2^31 elements in a stack, in one wide and in one tall matrix."""
+    y = gradient((4, 1000, 2000), 50, hip, BF16)
+    want = orthogonalize(y).float()
+    got = orthogonalize(y.repeat(280, 1, 1)).view(280, 4, 1000, 2000)
+    # the same products in other tiles: off by their error at most, and then by one step of bf16
+    dev = 6 * deviation(y, False).max() + want.abs() * torch.finfo(BF16).eps
+    for part in got:
+        assert bool(((part.float() - want).abs() <= dev).all())
+    del got
+    gen = torch.Generator(device=hip).manual_seed(6)
+    x = torch.randn(8192, 264000, generator=gen, device=hip, dtype=BF16)
+    assert x.numel() > 1 << 31
+    abc = (3.4445, -4.7750, 2.0315)
+    wide = orthogonalize(x, steps=1, coefficients=abc)
+    last = slice(-3000, None)  # far behind 2^31 in the last rows; every row of A depends on the whole of its row of X
+    z = x.float() / x.double().square().sum().sqrt().float()
+    g = torch.zeros(8192, 8192, device=hip, dtype=torch.float64)
+    for k in range(0, 264000, 24000):
+        part = z[:, k:k + 24000].double()
+        g += part @ part.mT.contiguous()
+    p = abc[1] * g + abc[2] * (g @ g)
+    for cols in (slice(0, 3000), last):
+        want = abc[0] * z[:, cols].double() + p @ z[:, cols].double()
+        # an entry is z's 3.4 times and sums of 22-bit products in fp32, far below a tenth of bf16's half step here
+        off = (wide[:, cols].double() - want).abs() - want.abs() * (torch.finfo(BF16).eps / 2 * 1.1)
+        assert bool((off <= want.abs().max() * 2.0 ** -16).all()), float(off.max())
+    tall = orthogonalize(x.mT.contiguous(), steps=1, coefficients=abc)
+    assert torch.equal(tall.mT, wide)
